@@ -176,15 +176,15 @@ def prepare(case, seed):
     s["row_start"] = torch.tensor(starts, dtype=torch.int32, device="cuda")
     s["kv_len"] = torch.tensor(kv, dtype=torch.int32, device="cuda")
     s["new"], s["rows"], s["kv_rows"] = new, starts[-1], kv
-    # the cache's memory: key codes, value codes, key scales, value scales
+    # the cache's memory: key codes, value codes (a byte holds the code plus 128), key scales, value scales
     codes, scales = pages * kh * PAGE * dp, pages * kh * (PAGE // b)
     mem = torch.empty(2 * codes + 8 * scales, dtype=torch.uint8, device="cuda")
     s["memory"] = mem
     for name, at in (("k_codes", 0), ("v_codes", codes)):
-        c = mem[at:at + codes].view(torch.int8)
-        for i in range(0, codes, 1 << 26):  # normal values, 127 the largest; in pieces, since the normals are four times as large
+        c = mem[at:at + codes]
+        for i in range(0, codes, 1 << 26):  # normal values, 127 the largest, plus 128; in pieces, since the normals are four times as large
             part = c[i:i + (1 << 26)]
-            part.copy_((rnd(part.numel()) * 36).clamp_(-127, 127).round_())
+            part.copy_((rnd(part.numel()) * 36).clamp_(-127, 127).round_().add_(128))
         s[name] = c
     for name, at in (("k_scale", 2 * codes), ("v_scale", 2 * codes + 4 * scales)):
         t = mem[at:at + 4 * scales].view(torch.float32)
@@ -316,12 +316,13 @@ def _plain_write(s):
         at = place[token][:, None]  # [sequences, 1, block, dp]
         who = begin_page[:, None, None, None]
         held = stored[who, heads[None, :, None, None], at]
-        again = torch.where(older[:, None, :, None], (held.to(torch.float32) * factor[:, :, None, None]).round().clamp(-127, 127).to(torch.int8), held)
+        moved = ((held.to(torch.float32) - 128) * factor[:, :, None, None]).round().clamp(-127, 127)
+        again = torch.where(older[:, None, :, None], (moved + 128).to(torch.uint8), held)
         stored[who, heads[None, :, None, None], at] = again
         # the new tokens
         mine = fresh[page, :, slot // b][:, :, None]
-        q = torch.where(mine > 0, x / mine, torch.zeros_like(x)).round().clamp(-127, 127).to(torch.int8)
-        stored[page[:, None, None], heads[None, :, None], place[slot][:, None, :dim]] = q
+        q = torch.where(mine > 0, x / mine, torch.zeros_like(x)).round().clamp(-127, 127)
+        stored[page[:, None, None], heads[None, :, None], place[slot][:, None, :dim]] = (q + 128).to(torch.uint8)
         flat.copy_(fresh)
     k, v = _plain_read(s)
     return k, v, s["k_scale"], s["v_scale"]
@@ -332,8 +333,8 @@ def _plain_read(s):
     kh, b, dim, dp = case["kv_heads"], case["block"], case["dim"], _row_dim(case["dim"])
     seq, pos = _rows_at(s["back"], s["kv_rows"])
     page, slot = s["pages"].to(torch.int64)[seq, pos // PAGE], pos % PAGE
-    k = _key_values(s["k_codes"], kh, dp)[page, :, slot, :dim].to(torch.float32) * s["k_scale"][page, :, slot // b][:, :, None]
-    v = _value_values(s["v_codes"], kh, dp)[page, :, slot, :dim].to(torch.float32) * s["v_scale"][page, :, slot // b][:, :, None]
+    k = _key_values(s["k_codes"], kh, dp)[page, :, slot, :dim].to(torch.float32).sub(128) * s["k_scale"][page, :, slot // b][:, :, None]
+    v = _value_values(s["v_codes"], kh, dp)[page, :, slot, :dim].to(torch.float32).sub(128) * s["v_scale"][page, :, slot // b][:, :, None]
     return k.to(TYPES[case["type"]]), v.to(TYPES[case["type"]])
 
 
@@ -345,7 +346,7 @@ def _plain_attend(s):
     pick = s["pages"].to(torch.int64).reshape(-1)
 
     def values(codes, scale, order):
-        x = order(codes.view(-1, kh, PAGE * dp)[pick], kh, dp)[..., :dim].to(torch.float32)
+        x = order(codes.view(-1, kh, PAGE * dp)[pick], kh, dp)[..., :dim].to(torch.float32) - 128
         x = x * scale[pick].repeat_interleave(b, -1)[..., None]
         return x.view(seqs, table, kh, PAGE, dim).permute(0, 2, 1, 3, 4).reshape(seqs, kh, longest, dim)
 
@@ -402,7 +403,7 @@ def _cached(s, i, count):
     pages = s["pages"][i, : -(-count // PAGE)].long()
     got = []
     for codes, scale, index in zip((s["k_codes"], s["v_codes"]), (s["k_scale"], s["v_scale"]), _token_index(dim, dp)):
-        c = codes.view(-1, kh, PAGE * dp)[pages][:, :, index.reshape(-1)].view(len(pages), kh, PAGE, dim).double()
+        c = codes.view(-1, kh, PAGE * dp)[pages][:, :, index.reshape(-1)].view(len(pages), kh, PAGE, dim).double() - 128
         c = c * scale[pages].double().repeat_interleave(b, 2)[..., None]
         got.append(c.transpose(0, 1).reshape(kh, -1, dim)[:, :count])
     return got
@@ -457,7 +458,7 @@ def _exact_write(s):
                 safe = torch.where(s1 > 0, s1, torch.ones_like(s1))
                 q = (mine / safe[None, :, None]).float().double().round().clamp(-127, 127)
                 slots = torch.arange(start % PAGE, start % PAGE + old, device="cuda")
-                kept = stored[page][:, place[slots].reshape(-1)].view(kh, old, dim).transpose(0, 1).double()
+                kept = stored[page][:, place[slots].reshape(-1)].view(kh, old, dim).transpose(0, 1).double() - 128
                 kept = (kept * (s0 / safe).float().double()[None, :, None]).float().double().round().clamp(-127, 127)
                 rows.append(torch.cat([kept, q]) * s1[None, :, None])
                 scale[page, :, blk] = s1
