@@ -111,8 +111,8 @@ int mi_qmm_vec_dot_type(int weight_type);
  *      ROCR_VISIBLE_DEVICES, /root/reference/ml/device.go:688-735); 0 is the normal value. */
 int mi_qmm_init(int device_ordinal, mi_qmm_ctx **out);
 void mi_qmm_destroy(mi_qmm_ctx *ctx);
-/* run on a caller-owned hipStream_t (e.g. the framework's current stream); NULL restores the
- * ctx's own stream.  The ctx never destroys a caller stream.  The call waits for the work queued on
+/* run on a caller-owned hipStream_t (e.g. the framework's current stream; hipStreamLegacy for HIP's
+ * default stream); NULL restores the ctx's own stream.  The ctx never destroys a caller stream.  The call waits for the work queued on
  * the previous stream.  With device pointers the product entry points only queue kernels once the
  * ctx's scratch buffers have reached their size (first call of a shape), so such calls may be
  * captured into a HIP graph on the caller's stream after one eager call. */
@@ -316,6 +316,97 @@ int mi_qmm_mulmat_id_swiglu(mi_qmm_ctx *ctx, const mi_qmm_weight *w_gate, const 
 int mi_qmm_mulmat_id_produced(mi_qmm_ctx *ctx, const mi_qmm_weight *w, int n_expert, int producer,
                               const float *aux, float eps, const float *x, int b_cols, const int32_t *ids,
                               int n_used, int64_t n_tokens, float *y, int location);
+
+/* ---- the attention side of a decoder layer: what stands between the q / k / v products and the o product.
+ *      Rotation, cache and attention take activations of type MI_QMM_TYPE_F32, _F16 or _BF16 (the products' own are f32);
+ *      sums, softmax statistics and norms are fp32 and every result is rounded once.  Row pointers are 16-byte aligned
+ *      and row strides (elements from one row to the next, at least a row's values) whole 16-byte pieces in bytes;
+ *      head_dim is a multiple of 8 up to 256; anything else is MI_QMM_ERR_INVALID or _UNSUPPORTED.  `location` covers
+ *      every pointer of a call, those inside the structs included; a cache is always device memory. */
+
+/* Norms of queries and keys for each head and the rotation by position, in one pass:
+ *     y = x / sqrt(mean(x^2) + eps) * weight     over the head_dim values of a head; left out where the weight is NULL
+ *     (a, b) -> mscale * (a cos t - b sin t, a sin t + b cos t),  t = pos[row] * freqs[i]   for the pairs i < n_rot / 2
+ * with (a, b) = (y[i], y[i + n_rot / 2]) for MI_QMM_ROPE_HALVES and (y[2 i], y[2 i + 1]) for MI_QMM_ROPE_ADJACENT.  Values
+ * from n_rot on (a multiple of 8, 0 for no rotation) are not rotated.  freqs: n_rot / 2 doubles, radians per position;
+ * angles are formed and reduced in 64 bits. */
+enum { MI_QMM_ROPE_HALVES = 0, MI_QMM_ROPE_ADJACENT = 1 };
+typedef struct mi_qmm_qk_heads {
+    int type;                            /* of q, k and the outputs */
+    int n_heads, n_kv_heads, head_dim;   /* n_kv_heads = 0: there is no k */
+    int n_rot, pairing;
+    float eps, mscale;
+    const float *q_weight, *k_weight;    /* [head_dim] or NULL */
+    const double *freqs;                 /* [n_rot / 2] */
+} mi_qmm_qk_heads;
+/* q [n][n_heads][head_dim], k [n][n_kv_heads][head_dim], pos int32 [n]; q_out / k_out may be q / k themselves (same
+ * pointer and stride) and may not overlap them otherwise (rows of one joined buffer interleave without overlapping). */
+int mi_qmm_qk_norm_rope(mi_qmm_ctx *ctx, const mi_qmm_qk_heads *heads, const void *q, int64_t q_stride, const void *k,
+                        int64_t k_stride, const int32_t *pos, int64_t n, void *q_out, int64_t q_out_stride, void *k_out,
+                        int64_t k_out_stride, int location);
+/* Fills freqs (HOST memory, n_rot / 2 doubles) and mscale; needs no GPU.  freq_i = base^(-2 i / n_rot) / factors[i]
+ * (factors may be NULL), times freq_scale (linear scaling); with ext_factor != 0 the published YaRN rule: dimensions that
+ * turn more than beta_fast times within n_ctx_orig positions keep their frequency, those below beta_slow turns take the
+ * scaled one, a ramp between; mscale = attn_factor * (1 + 0.1 ln(1 / freq_scale)).  Without it mscale = attn_factor. */
+int mi_qmm_rope_freqs(int n_rot, double base, double freq_scale, double ext_factor, double attn_factor, double beta_fast,
+                      double beta_slow, int n_ctx_orig, const float *factors, double *freqs, float *mscale);
+
+/* A key/value cache in 8 bits: pages of MI_QMM_KV_PAGE tokens; one fp32 scale for keys and one for values per `block`
+ * tokens (16, 32 or 64) and head.  The code of x is the whole number nearest to x / scale, -127..127.
+ * memory NULL: the library allocates (and zeroes) the cache's device memory.  Otherwise it is the caller's, device memory
+ * of mi_qmm_kv_bytes() bytes, 256-byte aligned, that outlives the handle: key codes, value codes, key scales, value
+ * scales, one after the other.  With dp = head_dim rounded up to 64, codes are bytes of code + 128,
+ * [n_pages][n_kv_heads][64 * dp], and lie inside a page and head at
+ *     key   (token t, dimension d):  (((t / 16 * (dp / 64) + d / 64) * 4 + d % 64 / 16) * 16 + t % 16) * 16 + d % 16
+ *     value (token t, dimension d):  ((d / 16 * 4 + t % 16 / 4) * 16 + d % 16) * 16 + t / 16 * 4 + t % 4
+ * and scales are f32 [n_pages][n_kv_heads][64 / block]. */
+#define MI_QMM_KV_PAGE 64
+typedef struct mi_qmm_kv mi_qmm_kv;
+int64_t mi_qmm_kv_bytes(int64_t n_pages, int n_kv_heads, int head_dim, int block); /* -1: no such cache */
+int mi_qmm_kv_create(mi_qmm_ctx *ctx, int64_t n_pages, int n_kv_heads, int head_dim, int block, void *memory, mi_qmm_kv **out);
+void mi_qmm_kv_free(mi_qmm_kv *kv);
+
+/* The sequences of a step.  Rows (of k, v, q, out) belong to sequence s from row_start[s] to row_start[s + 1] - 1 and are
+ * its LAST tokens: kv_len[s] counts the tokens of the sequence with them, so row i of r rows is at position
+ * kv_len[s] - r + i.  Token p lies in page pages[s][p / 64], slot p % 64.  Rows that belong to no sequence (behind
+ * row_start[n_seqs], padding) are neither read nor written.
+ * With host arrays a page that is needed and outside 0..n_pages - 1, a length beyond the table, rows beyond the length or
+ * row_start that falls or leaves 0..n is MI_QMM_ERR_INVALID.  With device arrays the call cannot see them: tokens of such
+ * a page (or beyond the table) are not written, read back as NaN, and make every row that sees them NaN; rows whose
+ * row_start is wrong, or whose position is negative, are left alone by write and read. */
+typedef struct mi_qmm_batch {
+    int n_seqs, max_pages;
+    const int32_t *row_start; /* [n_seqs + 1] */
+    const int32_t *kv_len;    /* [n_seqs] */
+    const int32_t *pages;     /* [n_seqs][max_pages] */
+} mi_qmm_batch;
+/* Quantizes the rows into their places.  A block whose first token is written takes the scale of this call's values,
+ * max |x| * (1 / 127); a block that goes on keeps its scale unless that is larger, and then its older codes are rounded
+ * anew against the larger one.  A value that is not finite makes the block's scale NaN until its first token is written
+ * again.  The pages written must belong to one sequence of the call each (host arrays: MI_QMM_ERR_INVALID otherwise;
+ * device arrays: such a page's content is undefined).  k, v [n][n_kv_heads][head_dim]. */
+int mi_qmm_kv_write(mi_qmm_ctx *ctx, mi_qmm_kv *kv, const mi_qmm_batch *batch, int type, const void *k, int64_t k_stride,
+                    const void *v, int64_t v_stride, int64_t n, int location);
+/* Reads the rows' tokens back: code * scale, rounded to the type.  row_start may name any number of a sequence's last
+ * tokens, all of them included. */
+int mi_qmm_kv_read(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *batch, int type, void *k, int64_t k_stride,
+                   void *v, int64_t v_stride, int64_t n, int location);
+
+/* Attention of the rows over the cache:
+ *     out = sum_j w_j v_j / (sum_j w_j + exp(sink)),  w_j = exp(z_j),  z_j = cap(scale * q . k_j),  cap(z) = c tanh(z / c)
+ * over the tokens j of the row's sequence with j <= its position (causal) and j > its position - window (window > 0).
+ * Query head h reads key/value head h / (n_heads / n_kv_heads).  sinks: one logit per query head that takes part in the
+ * sum only; softcap 0: no cap.  A row that sees no token gives zeros.  f32 calls carry f32 accuracy (queries and
+ * probabilities are split into two halves each); the 16-bit types take probabilities of 11 bits.  The rows' own tokens
+ * are to be written first (mi_qmm_kv_write on the same batch).  q, out [n][n_heads][head_dim], not overlapping. */
+typedef struct mi_qmm_attn {
+    int type, n_heads;
+    float scale, softcap;
+    int causal, window;
+    const float *sinks; /* [n_heads] or NULL */
+} mi_qmm_attn;
+int mi_qmm_attention(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *batch, const mi_qmm_attn *how, const void *q,
+                     int64_t q_stride, void *out, int64_t out_stride, int64_t n, int location);
 
 /* ---- two-phase form: quantize once, multiply by several weights (gate and up, or q/k/v, share
  *      one x).  In ggml's graph the from_float step belongs to each mul_mat node; a backend that

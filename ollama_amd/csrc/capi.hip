@@ -2,6 +2,7 @@
 // Everything that computes runs on the GPU; there is no CPU fallback in this file.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -79,6 +80,13 @@ struct mi_qmm_weight {
     // for the streaming kernel at one or two activation rows -- against x itself, not [x | x]
     bool has_native = false;
     DevWeight native{};
+};
+
+struct mi_qmm_kv {
+    int device = 0;
+    void *base = nullptr;
+    bool owned = false;
+    DevKv dev{};
 };
 
 struct mi_qmm_gguf {
@@ -1970,6 +1978,342 @@ int mi_qmm_gguf_upload(mi_qmm_ctx *ctx, const mi_qmm_gguf *f, int64_t index, mi_
     // an expert stack [K, M, E] is E matrices of M rows one after the other: the same bytes as [K, M*E]
     const int64_t m = (int64_t)t.dims[1] * (t.n_dims == 3 ? (int64_t)t.dims[2] : 1);
     return mi_qmm_weight_upload(ctx, (int)t.type, f->file.tensor_data(t), (int64_t)t.dims[0], m, MI_QMM_HOST, out);
+}
+
+}  // extern "C"
+
+// ---- rotation, cache, attention -------------------------------------------------------------------
+namespace {
+
+int value_size(int type) { return type == T_F32 ? 4 : type == T_F16 || type == T_BF16 ? 2 : 0; }
+
+int check_values(int type, int64_t n, int location) {
+    if (!value_size(type)) return fail(MI_QMM_ERR_UNSUPPORTED, "type %d is not F32 (0), F16 (1) or BF16 (30)", type);
+    if (n < 0) return fail(MI_QMM_ERR_INVALID, "n=%lld must be non-negative", (long long)n);
+    if (n > (1 << 24)) return fail(MI_QMM_ERR_UNSUPPORTED, "n=%lld: at most 2^24 rows", (long long)n);
+    if (location != MI_QMM_HOST && location != MI_QMM_DEVICE)
+        return fail(MI_QMM_ERR_INVALID, "location must be MI_QMM_HOST or MI_QMM_DEVICE");
+    return MI_QMM_OK;
+}
+
+// rows of heads x head_dim values
+int check_rows(const char *name, const void *p, int64_t stride, int heads, int head_dim, int type, int location) {
+    if (!p) return fail(MI_QMM_ERR_INVALID, "%s is NULL", name);
+    if (stride < (int64_t)heads * head_dim)
+        return fail(MI_QMM_ERR_INVALID, "%s: a stride of %lld is less than the row's %lld values", name, (long long)stride,
+                    (long long)heads * head_dim);
+    if (stride > (1ll << 31)) return fail(MI_QMM_ERR_UNSUPPORTED, "%s: a stride of %lld values", name, (long long)stride);
+    if (stride * value_size(type) % 16) return fail(MI_QMM_ERR_INVALID, "%s: a stride of %lld values is no multiple of 16 bytes", name, (long long)stride);
+    if (location == MI_QMM_DEVICE && (uintptr_t)p % 16) return fail(MI_QMM_ERR_INVALID, "%s is not 16-byte aligned", name);
+    return MI_QMM_OK;
+}
+
+size_t span(int64_t n, int64_t stride, int heads, int head_dim, int type) {  // bytes from the first value to the last
+    return n ? (size_t)((n - 1) * stride + (int64_t)heads * head_dim) * value_size(type) : 0;
+}
+
+// rows of heads x head_dim values in memory
+struct Rows {
+    const void *p;
+    int64_t stride;
+    int heads;
+    size_t bytes;
+};
+
+// whether two sets of rows share memory; the rows of one joined buffer ([n][q | k | v]) interleave without sharing any
+bool share(const Rows &a, const Rows &b, int head_dim, int type) {
+    const char *x = (const char *)a.p, *y = (const char *)b.p;
+    if (x >= y + b.bytes || y >= x + a.bytes) return false;
+    const int64_t size = value_size(type), s = a.stride, d = y - x;
+    if (s != b.stride || d % size) return true;
+    const int64_t m = (d / size % s + s) % s;  // where b's rows start inside a's
+    return m < (int64_t)a.heads * head_dim || m + (int64_t)b.heads * head_dim > s;
+}
+
+// host copies of output rows: the rows alone, not what lies between them
+hipError_t rows_to_host(void *host, const void *dev, int64_t n, int64_t stride, int heads, int head_dim, int type, hipStream_t s) {
+    const size_t size = value_size(type), pitch = (size_t)stride * size;
+    return hipMemcpy2DAsync(host, pitch, dev, pitch, (size_t)heads * head_dim * size, (size_t)n, hipMemcpyDeviceToHost, s);
+}
+
+int check_kv(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *b) {
+    if (!kv || !b) return fail(MI_QMM_ERR_INVALID, "kv or batch is NULL");
+    if (b->n_seqs < 0 || b->max_pages < 1 || b->max_pages > (1 << 24) || b->n_seqs > (1 << 24))
+        return fail(MI_QMM_ERR_INVALID, "n_seqs=%d max_pages=%d", b->n_seqs, b->max_pages);
+    if (b->n_seqs && (!b->row_start || !b->kv_len || !b->pages)) return fail(MI_QMM_ERR_INVALID, "row_start, kv_len or pages is NULL");
+    if (kv->device != ctx->device) return fail(MI_QMM_ERR_INVALID, "kv and ctx are on different devices");
+    return MI_QMM_OK;
+}
+
+// host arrays are looked at: every page that the call needs exists; each written page belongs to one sequence
+int check_host_batch(const mi_qmm_kv *kv, const mi_qmm_batch *b, int64_t n, bool whole, bool writes) {
+    uint8_t *seen = nullptr;
+    if (writes) {
+        seen = new (std::nothrow) uint8_t[(size_t)kv->dev.n_pages]();
+        if (!seen) return fail(MI_QMM_ERR_NOMEM, "host allocation failed");
+    }
+    int rc = MI_QMM_OK;
+    for (int s = 0; s < b->n_seqs && !rc; s++) {
+        const int64_t from = b->row_start[s], to = b->row_start[s + 1], len = b->kv_len[s];
+        if (from < 0 || to < from || to > n)
+            rc = fail(MI_QMM_ERR_INVALID, "rows %lld..%lld of sequence %d are outside 0..%lld", (long long)from, (long long)to, s, (long long)n);
+        else if (len < 0 || len > (int64_t)b->max_pages * KV_PAGE || to - from > len)
+            rc = fail(MI_QMM_ERR_INVALID, "sequence %d: %lld rows, %lld tokens, a table of %d pages", s, (long long)(to - from), (long long)len, b->max_pages);
+        if (rc || to == from) continue;
+        for (int64_t p = whole ? 0 : (len - (to - from)) / KV_PAGE; p * KV_PAGE < len && !rc; p++) {
+            const int64_t page = b->pages[(int64_t)s * b->max_pages + p];
+            if (page < 0 || page >= kv->dev.n_pages)
+                rc = fail(MI_QMM_ERR_INVALID, "sequence %d: page %lld is outside 0..%lld", s, (long long)page, (long long)kv->dev.n_pages - 1);
+            else if (writes && seen[page]++)
+                rc = fail(MI_QMM_ERR_INVALID, "page %lld is written twice", (long long)page);
+        }
+    }
+    delete[] seen;
+    return rc;
+}
+
+// the batch's arrays as device pointers; d: [row_start, kv_len, pages] staged
+DevBatch dev_batch(const mi_qmm_batch *b, void *const *d, int64_t n) {
+    return DevBatch{(const int32_t *)d[0], (const int32_t *)d[1], (const int32_t *)d[2], b->n_seqs, b->max_pages, (int)n};
+}
+
+void batch_sources(const mi_qmm_batch *b, const void **src, size_t *bytes) {
+    src[0] = b->row_start; bytes[0] = ((size_t)b->n_seqs + 1) * 4;
+    src[1] = b->kv_len;    bytes[1] = (size_t)b->n_seqs * 4;
+    src[2] = b->pages;     bytes[2] = (size_t)b->n_seqs * b->max_pages * 4;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mi_qmm_rope_freqs(int n_rot, double base, double freq_scale, double ext_factor, double attn_factor, double beta_fast,
+                      double beta_slow, int n_ctx_orig, const float *factors, double *freqs, float *mscale) {
+    if (n_rot < 2 || n_rot % 2) return fail(MI_QMM_ERR_INVALID, "n_rot=%d must be even and positive", n_rot);
+    if (!(base > 1.0) || !(freq_scale > 0.0)) return fail(MI_QMM_ERR_INVALID, "base=%g must be above 1 and freq_scale=%g positive", base, freq_scale);
+    if (!freqs || !mscale) return fail(MI_QMM_ERR_INVALID, "freqs or mscale is NULL");
+    const bool yarn = ext_factor != 0.0;
+    if (yarn && (n_ctx_orig < 1 || !(beta_fast > 0.0) || !(beta_slow > 0.0)))
+        return fail(MI_QMM_ERR_INVALID, "n_ctx_orig=%d beta_fast=%g beta_slow=%g must be positive", n_ctx_orig, beta_fast, beta_slow);
+    double low = 0.0, high = 0.0;
+    if (yarn) {
+        // the dimension that turns beta times within n_ctx_orig positions: n_ctx_orig * base^(-2 i / n_rot) = 2 pi beta
+        const double two_pi = 6.283185307179586477, span_of = n_rot / (2.0 * log(base));
+        low = fmax(floor(span_of * log(n_ctx_orig / (beta_fast * two_pi))), 0.0);
+        high = fmin(ceil(span_of * log(n_ctx_orig / (beta_slow * two_pi))), n_rot - 1.0);
+    }
+    for (int i = 0; i < n_rot / 2; i++) {
+        double f = pow(base, -2.0 * i / n_rot);
+        if (factors) f /= (double)factors[i];
+        double keep = 0.0;  // share of the unscaled frequency
+        if (yarn) keep = (1.0 - fmin(fmax((i - low) / fmax(0.001, high - low), 0.0), 1.0)) * ext_factor;
+        freqs[i] = f * (freq_scale * (1.0 - keep) + keep);
+    }
+    *mscale = (float)(attn_factor * (yarn ? 1.0 + 0.1 * log(1.0 / freq_scale) : 1.0));
+    return MI_QMM_OK;
+}
+
+int mi_qmm_qk_norm_rope(mi_qmm_ctx *ctx, const mi_qmm_qk_heads *p, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                        const int32_t *pos, int64_t n, void *q_out, int64_t q_out_stride, void *k_out, int64_t k_out_stride,
+                        int location) {
+    if (!p) return fail(MI_QMM_ERR_INVALID, "heads is NULL");
+    int rc = check_values(p->type, n, location);
+    if (rc) return rc;
+    if (p->n_heads < 1 || p->n_kv_heads < 0 || p->n_heads > 65535 || p->n_kv_heads > 65535)
+        return fail(MI_QMM_ERR_INVALID, "n_heads=%d n_kv_heads=%d", p->n_heads, p->n_kv_heads);
+    if (p->head_dim < 8 || p->head_dim > 256 || p->head_dim % 8)
+        return fail(MI_QMM_ERR_UNSUPPORTED, "head_dim=%d is no multiple of 8 from 8 to 256", p->head_dim);
+    if (p->n_rot < 0 || p->n_rot > p->head_dim || p->n_rot % 8)
+        return fail(MI_QMM_ERR_UNSUPPORTED, "n_rot=%d is no multiple of 8 from 0 to head_dim=%d", p->n_rot, p->head_dim);
+    if (p->pairing != MI_QMM_ROPE_HALVES && p->pairing != MI_QMM_ROPE_ADJACENT) return fail(MI_QMM_ERR_INVALID, "pairing=%d", p->pairing);
+    if (!(p->eps >= 0.f)) return fail(MI_QMM_ERR_INVALID, "eps must be non-negative");
+    if ((rc = check_ctx(ctx))) return rc;
+    if (n == 0) return MI_QMM_OK;
+    const int dim = p->head_dim, heads[2] = {p->n_heads, p->n_kv_heads};
+    const void *in[2] = {q, k};
+    void *out[2] = {q_out, k_out};
+    const int64_t is[2] = {q_stride, k_stride}, os[2] = {q_out_stride, k_out_stride};
+    static const char *const in_name[2] = {"q", "k"}, *const out_name[2] = {"q_out", "k_out"};
+    const int both = p->n_kv_heads ? 2 : 1;
+    for (int i = 0; i < both; i++) {
+        if ((rc = check_rows(in_name[i], in[i], is[i], heads[i], dim, p->type, location))) return rc;
+        if ((rc = check_rows(out_name[i], out[i], os[i], heads[i], dim, p->type, location))) return rc;
+    }
+    if (!pos || (p->n_rot && !p->freqs)) return fail(MI_QMM_ERR_INVALID, "pos or freqs is NULL");
+    const void *src[8];
+    size_t bytes[8];
+    for (int i = 0; i < 2; i++) {
+        src[i] = i < both ? in[i] : nullptr;          bytes[i] = i < both ? span(n, is[i], heads[i], dim, p->type) : 0;
+        src[6 + i] = i < both ? out[i] : nullptr;     bytes[6 + i] = i < both ? span(n, os[i], heads[i], dim, p->type) : 0;
+    }
+    // an output may be its own input, row for row; any other sharing would be read after it was written
+    for (int i = 0; i < both; i++)
+        for (int j = 0; j < both; j++) {
+            if (i == j && in[i] == out[j] && is[i] == os[j]) continue;
+            if (share({in[i], is[i], heads[i], bytes[i]}, {out[j], os[j], heads[j], bytes[6 + j]}, dim, p->type))
+                return fail(MI_QMM_ERR_INVALID, "%s overlaps %s", out_name[j], in_name[i]);
+        }
+    if (both == 2 && share({out[0], os[0], heads[0], bytes[6]}, {out[1], os[1], heads[1], bytes[7]}, dim, p->type))
+        return fail(MI_QMM_ERR_INVALID, "k_out overlaps q_out");
+    src[2] = pos;         bytes[2] = (size_t)n * 4;
+    src[3] = p->q_weight; bytes[3] = p->q_weight ? (size_t)dim * 4 : 0;
+    src[4] = p->k_weight; bytes[4] = p->k_weight ? (size_t)dim * 4 : 0;
+    src[5] = p->freqs;    bytes[5] = (size_t)p->n_rot * 4;
+    void *d[8];
+    if ((rc = stage_in(ctx, location, src, bytes, 6, 8, d))) return rc;
+    const RopeDesc desc{p->q_weight ? (const float *)d[3] : nullptr, p->k_weight ? (const float *)d[4] : nullptr, (const double *)d[5],
+                        p->eps, p->mscale, p->n_heads, p->n_kv_heads, dim, p->n_rot, p->pairing == MI_QMM_ROPE_HALVES};
+    HIP_TRY(launch_qk_norm_rope(p->type, desc, d[0], q_stride, d[1], k_stride, (const int32_t *)d[2], (int)n, d[6], q_out_stride,
+                                d[7], k_out_stride, ctx->stream));
+    if (location == MI_QMM_HOST) {
+        for (int i = 0; i < both; i++) HIP_TRY(rows_to_host(out[i], d[6 + i], n, os[i], heads[i], dim, p->type, ctx->stream));
+        HIP_TRY(hipStreamSynchronize(ctx->stream));
+    }
+    return MI_QMM_OK;
+}
+
+int64_t mi_qmm_kv_bytes(int64_t n_pages, int n_kv_heads, int head_dim, int block) {
+    if (n_pages < 1 || n_pages > INT32_MAX || n_kv_heads < 1 || n_kv_heads > 65535 || head_dim < 8 || head_dim > 256 || head_dim % 8 ||
+        (block != 16 && block != 32 && block != 64))
+        return -1;
+    const int64_t dp = (head_dim + 63) / 64 * 64;
+    return n_pages * n_kv_heads * (2 * KV_PAGE * dp + 8 * (KV_PAGE / block));
+}
+
+int mi_qmm_kv_create(mi_qmm_ctx *ctx, int64_t n_pages, int n_kv_heads, int head_dim, int block, void *memory, mi_qmm_kv **out) {
+    if (!out) return fail(MI_QMM_ERR_INVALID, "out is NULL");
+    *out = nullptr;
+    const int64_t bytes = mi_qmm_kv_bytes(n_pages, n_kv_heads, head_dim, block);
+    if (bytes < 0)
+        return fail(MI_QMM_ERR_UNSUPPORTED, "n_pages=%lld n_kv_heads=%d head_dim=%d block=%d: head_dim is a multiple of 8 up to 256, block 16, 32 or 64",
+                    (long long)n_pages, n_kv_heads, head_dim, block);
+    if ((uintptr_t)memory % 256) return fail(MI_QMM_ERR_INVALID, "memory is not 256-byte aligned");
+    int rc = check_ctx(ctx);
+    if (rc) return rc;
+    mi_qmm_kv *kv = new (std::nothrow) mi_qmm_kv();
+    if (!kv) return fail(MI_QMM_ERR_NOMEM, "host allocation failed");
+    kv->device = ctx->device;
+    kv->base = memory;
+    if (!memory) {
+        hipError_t e = hipMalloc(&kv->base, (size_t)bytes);
+        if (e != hipSuccess) {
+            delete kv;
+            return fail(MI_QMM_ERR_NOMEM, "hipMalloc(%lld) for a cache: %s", (long long)bytes, hipGetErrorString(e));
+        }
+        kv->owned = true;
+        e = hipMemsetAsync(kv->base, 0, (size_t)bytes, ctx->stream);
+        if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+        if (e != hipSuccess) {
+            (void)hipFree(kv->base);
+            delete kv;
+            return fail(MI_QMM_ERR_HIP, "clearing a cache: %s", hipGetErrorString(e));
+        }
+    }
+    DevKv &c = kv->dev;
+    c.n_pages = n_pages; c.kv_heads = n_kv_heads; c.head_dim = head_dim; c.dp = (head_dim + 63) / 64 * 64;
+    c.block = block; c.per = KV_PAGE / block;
+    const int64_t codes = n_pages * n_kv_heads * KV_PAGE * c.dp;
+    c.k = (uint8_t *)kv->base;
+    c.v = c.k + codes;
+    c.ks = (float *)(c.v + codes);
+    c.vs = c.ks + n_pages * n_kv_heads * c.per;
+    *out = kv;
+    return MI_QMM_OK;
+}
+
+void mi_qmm_kv_free(mi_qmm_kv *kv) {
+    if (!kv) return;
+    if (kv->owned && hipSetDevice(kv->device) == hipSuccess) {
+        (void)hipDeviceSynchronize();
+        (void)hipFree(kv->base);
+    }
+    delete kv;
+}
+
+int mi_qmm_kv_write(mi_qmm_ctx *ctx, mi_qmm_kv *kv, const mi_qmm_batch *b, int type, const void *k, int64_t k_stride, const void *v,
+                    int64_t v_stride, int64_t n, int location) {
+    int rc = check_values(type, n, location);
+    if (rc || (rc = check_ctx(ctx)) || (rc = check_kv(ctx, kv, b))) return rc;
+    if (n == 0 || b->n_seqs == 0) return MI_QMM_OK;
+    const DevKv &c = kv->dev;
+    if ((rc = check_rows("k", k, k_stride, c.kv_heads, c.head_dim, type, location)) ||
+        (rc = check_rows("v", v, v_stride, c.kv_heads, c.head_dim, type, location)))
+        return rc;
+    if (location == MI_QMM_HOST && (rc = check_host_batch(kv, b, n, false, true))) return rc;
+    const void *src[5];
+    size_t bytes[5];
+    batch_sources(b, src, bytes);
+    src[3] = k; bytes[3] = span(n, k_stride, c.kv_heads, c.head_dim, type);
+    src[4] = v; bytes[4] = span(n, v_stride, c.kv_heads, c.head_dim, type);
+    void *d[5];
+    if ((rc = stage_in(ctx, location, src, bytes, 5, 5, d))) return rc;
+    HIP_TRY(launch_kv_write(c, dev_batch(b, d, n), type, d[3], d[4], k_stride, v_stride, ctx->stream));
+    if (location == MI_QMM_HOST) HIP_TRY(hipStreamSynchronize(ctx->stream));
+    return MI_QMM_OK;
+}
+
+int mi_qmm_kv_read(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *b, int type, void *k, int64_t k_stride, void *v,
+                   int64_t v_stride, int64_t n, int location) {
+    int rc = check_values(type, n, location);
+    if (rc || (rc = check_ctx(ctx)) || (rc = check_kv(ctx, kv, b))) return rc;
+    if (n == 0 || b->n_seqs == 0) return MI_QMM_OK;
+    const DevKv &c = kv->dev;
+    if ((rc = check_rows("k", k, k_stride, c.kv_heads, c.head_dim, type, location)) ||
+        (rc = check_rows("v", v, v_stride, c.kv_heads, c.head_dim, type, location)))
+        return rc;
+    if (location == MI_QMM_HOST && (rc = check_host_batch(kv, b, n, false, false))) return rc;
+    const void *src[5];
+    size_t bytes[5];
+    batch_sources(b, src, bytes);
+    src[3] = k; bytes[3] = span(n, k_stride, c.kv_heads, c.head_dim, type);
+    src[4] = v; bytes[4] = span(n, v_stride, c.kv_heads, c.head_dim, type);
+    void *d[5];
+    if (share({k, k_stride, c.kv_heads, bytes[3]}, {v, v_stride, c.kv_heads, bytes[4]}, c.head_dim, type))
+        return fail(MI_QMM_ERR_INVALID, "k and v overlap");
+    if ((rc = stage_in(ctx, location, src, bytes, 5, 5, d))) return rc;  // outputs too: rows of no sequence stay as they are
+    HIP_TRY(launch_kv_read(c, dev_batch(b, d, n), type, d[3], d[4], k_stride, v_stride, ctx->stream));
+    if (location == MI_QMM_HOST) {
+        HIP_TRY(rows_to_host(k, d[3], n, k_stride, c.kv_heads, c.head_dim, type, ctx->stream));
+        HIP_TRY(rows_to_host(v, d[4], n, v_stride, c.kv_heads, c.head_dim, type, ctx->stream));
+        HIP_TRY(hipStreamSynchronize(ctx->stream));
+    }
+    return MI_QMM_OK;
+}
+
+int mi_qmm_attention(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *b, const mi_qmm_attn *p, const void *q, int64_t q_stride,
+                     void *out, int64_t out_stride, int64_t n, int location) {
+    if (!p) return fail(MI_QMM_ERR_INVALID, "how is NULL");
+    int rc = check_values(p->type, n, location);
+    if (rc || (rc = check_ctx(ctx)) || (rc = check_kv(ctx, kv, b))) return rc;
+    const DevKv &c = kv->dev;
+    if (p->n_heads < 1 || p->n_heads > 65535 || p->n_heads % c.kv_heads)
+        return fail(MI_QMM_ERR_INVALID, "n_heads=%d is no multiple of the cache's %d heads", p->n_heads, c.kv_heads);
+    if (!(p->softcap >= 0.f) || p->window < 0) return fail(MI_QMM_ERR_INVALID, "softcap=%g window=%d must be non-negative", (double)p->softcap, p->window);
+    if (n * (p->n_heads / c.kv_heads) > (1 << 27)) return fail(MI_QMM_ERR_UNSUPPORTED, "n=%lld rows of %d heads", (long long)n, p->n_heads);
+    if (n == 0 || b->n_seqs == 0) return MI_QMM_OK;
+    if ((rc = check_rows("q", q, q_stride, p->n_heads, c.head_dim, p->type, location)) ||
+        (rc = check_rows("out", out, out_stride, p->n_heads, c.head_dim, p->type, location)))
+        return rc;
+    if (location == MI_QMM_HOST && (rc = check_host_batch(kv, b, n, true, false))) return rc;
+    const void *src[6];
+    size_t bytes[6];
+    batch_sources(b, src, bytes);
+    src[3] = q;        bytes[3] = span(n, q_stride, p->n_heads, c.head_dim, p->type);
+    src[4] = p->sinks; bytes[4] = p->sinks ? (size_t)p->n_heads * 4 : 0;
+    src[5] = out;      bytes[5] = span(n, out_stride, p->n_heads, c.head_dim, p->type);
+    if (share({q, q_stride, p->n_heads, bytes[3]}, {out, out_stride, p->n_heads, bytes[5]}, c.head_dim, p->type))
+        return fail(MI_QMM_ERR_INVALID, "out overlaps q");
+    void *d[6];
+    if ((rc = stage_in(ctx, location, src, bytes, 6, 6, d))) return rc;  // out too: rows of no sequence stay as they are
+    const AttnDesc desc{p->type, p->n_heads, p->scale, p->softcap, p->causal, p->window, p->sinks ? (const float *)d[4] : nullptr};
+    const DevBatch db = dev_batch(b, d, n);
+    if ((rc = reserve(ctx, &ctx->ws_buf, &ctx->ws_cap, attn_workspace_floats(c, db, desc, ctx->num_cus) * 4))) return rc;
+    HIP_TRY(launch_attention(c, db, desc, d[3], q_stride, d[5], out_stride, (float *)ctx->ws_buf, ctx->num_cus, ctx->stream));
+    if (location == MI_QMM_HOST) {
+        HIP_TRY(rows_to_host(out, d[5], n, out_stride, p->n_heads, c.head_dim, p->type, ctx->stream));
+        HIP_TRY(hipStreamSynchronize(ctx->stream));
+    }
+    return MI_QMM_OK;
 }
 
 }  // extern "C"

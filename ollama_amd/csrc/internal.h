@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "formats.h"
+#include "kv_dev.h"
 #include "produce_dev.h"
 
 namespace miqmm {
@@ -201,5 +202,34 @@ bool plain_type(int type);
 int plain_kind(int type, int64_t K, int64_t M, int64_t N, int force = 0);
 size_t plain_convert_bytes(int type, int64_t K, int64_t N);
 hipError_t launch_plain(const DevWeight &w, const float *x, int64_t N, float *y, void *xc, int num_cus, hipStream_t s, int force = 0);
+
+// Norms of queries and keys per head and the rotation by position (rope.hip).  type: T_F32 / T_F16 / T_BF16; strides in
+// elements; rows and strides in whole 16-byte pieces; out may be in.
+struct RopeDesc {
+    const float *q_weight, *k_weight;  // [head_dim] or null: no norm
+    const double *freqs;               // [n_rot / 2] radians per position
+    float eps, mscale;
+    int n_heads, n_kv_heads, head_dim, n_rot;
+    bool halves;
+};
+hipError_t launch_qk_norm_rope(int type, const RopeDesc &d, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                               const int32_t *pos, int n, void *q_out, int64_t q_out_stride, void *k_out,
+                               int64_t k_out_stride, hipStream_t s);
+
+// The 8-bit key/value cache (kvcache.hip) and attention over it (attention.hip); b.n_rows > 0
+hipError_t launch_kv_write(const DevKv &c, const DevBatch &b, int type, const void *k, const void *v, int64_t k_stride,
+                           int64_t v_stride, hipStream_t s);
+hipError_t launch_kv_read(const DevKv &c, const DevBatch &b, int type, void *k, void *v, int64_t k_stride, int64_t v_stride,
+                          hipStream_t s);
+struct AttnDesc {
+    int type, n_heads;
+    float scale, softcap;  // softcap 0: none
+    int causal, window;    // window 0: none
+    const float *sinks;    // [n_heads] or null
+};
+// floats of workspace a call wants for the partial results of its splits (0: none)
+size_t attn_workspace_floats(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus);
+hipError_t launch_attention(const DevKv &c, const DevBatch &b, const AttnDesc &d, const void *q, int64_t q_stride, void *out,
+                            int64_t out_stride, float *workspace, int num_cus, hipStream_t s);
 
 }  // namespace miqmm

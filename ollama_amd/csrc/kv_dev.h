@@ -1,0 +1,78 @@
+// The 8-bit key/value cache as the kernels see it, and the description of a step's sequences.
+//
+// Memory of a cache (mi_qmm_kv_create): pages of 64 tokens; per page and key/value head 64 x dp key codes, then in a plane
+// of its own 64 x dp value codes, dp = the head dimension rounded up to 64.  A byte holds a code plus 128, so that zero
+// extended to 16 bits it is the subnormal half (code + 128) * 2^-24: the attention kernels widen codes with one byte
+// permute per pair and no conversion.  Both planes are in the order in which a wave loads matrix-core operands, every load
+// of a wave being 1 KiB in a row:
+//   key of token t, dimension d:   16-byte pieces [t / 16][d / 64][d % 64 / 16][t % 16], byte d % 16 of the piece
+//   value:                         16-byte pieces [d / 16][t % 16 / 4][d % 16],          byte 4 (t / 16) + t % 4
+// A lane's key piece is 16 dimensions of one token; its value piece 16 tokens of one dimension, the ones whose scores the
+// same lane group holds after the first product, so that the probabilities go into the second without any exchange.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace miqmm {
+
+constexpr int KV_PAGE = 64;
+
+struct DevKv {
+    uint8_t *k, *v;         // [n_pages][kv_heads][64 * dp]
+    float *ks, *vs;         // [n_pages][kv_heads][64 / block]
+    int64_t n_pages;
+    int kv_heads, head_dim, dp;
+    int block, per;         // tokens per scale, scales per page and head
+};
+
+struct DevBatch {
+    const int32_t *row_start;  // [n_seqs + 1]
+    const int32_t *kv_len;     // [n_seqs]
+    const int32_t *pages;      // [n_seqs][max_pages]
+    int n_seqs, max_pages;
+    int n_rows;
+};
+
+// rows of sequence s and the first of them; a range that is no part of 0..n_rows counts as none
+__device__ __forceinline__ int seq_rows(const DevBatch &b, int s, int &begin) {
+    begin = b.row_start[s];
+    const int end = b.row_start[s + 1];
+    return begin >= 0 && end <= b.n_rows && end > begin ? end - begin : 0;
+}
+
+// Work items numbered through the sequences, count(s) of them in sequence s: which sequence item `item` falls into and
+// its number there.  All lanes of a wave call it together; one round of loads per 64 sequences.
+template <class F>
+__device__ __forceinline__ bool find_item(int n_seqs, int item, F count, int &seq, int &local) {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (int s0 = 0; s0 < n_seqs; s0 += 64) {
+        const int s = s0 + lane;
+        const int c = s < n_seqs ? count(s) : 0;
+        int incl = c;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(incl, o);
+            if (lane >= o) incl += v;
+        }
+        const int total = __builtin_amdgcn_readlane(incl, 63);
+        if (item < base + total) {
+            const unsigned long long past = __ballot(base + incl > item);
+            const int at = __builtin_ctzll(past);
+            seq = s0 + at;
+            local = item - base - __builtin_amdgcn_readlane(incl - c, at);
+            return true;
+        }
+        base += total;
+    }
+    return false;
+}
+
+template <class T> struct Vec4 { using type = T __attribute__((ext_vector_type(4))); };
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
+__device__ __forceinline__ float to_f32(__bf16 v) { return (float)v; }
+
+}  // namespace miqmm

@@ -1,0 +1,285 @@
+// The 8-bit key/value cache: tokens quantized as they are written, and read back (layout: kv_dev.h).
+//
+// A block of tokens and a head share a scale s = max |x| / 127; codes are x / s rounded to the nearest whole number.  A
+// write that goes on in a partly filled block takes s = max(old s, new max / 127) and, where that grew, moves the older
+// codes to it: q -> round(q * (old s / s)).  A value that is not finite makes the scale NaN (and every token of the block
+// read as NaN) until a write starts the block anew.  All of it is fp32 arithmetic rounded operation by operation, so a
+// restatement gives the same bytes.
+//
+// Bound: memory.  One workgroup per page, head and plane.  Writing, a wave owns the tokens 16 m + 4 g + i (g its number) and
+// a lane dp / 64 neighbouring dimensions, so a row of a head is read in one piece, the block's maximum is one exchange
+// through LDS, and a lane holds whole 16-byte value pieces; key codes are turned into their pieces through LDS.
+#include "internal.h"
+#include "kv_dev.h"
+
+namespace miqmm {
+
+namespace {
+
+constexpr float PER127 = 0x1.020408p-7f;  // fl(1 / 127)
+
+// pages that the rows of sequence s touch, `first` their first token
+__device__ __forceinline__ int pages_touched(const DevBatch &b, int s, bool within_table, int &begin, int &n, int &first, int &len) {
+    n = seq_rows(b, s, begin);
+    len = b.kv_len[s];
+    first = len - n;
+    if (n == 0 || len <= 0) return 0;
+    int last = (len - 1) / KV_PAGE;
+    if (within_table) last = min(last, b.max_pages - 1);
+    return max(0, last - max(first, 0) / KV_PAGE + 1);
+}
+
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+    return v;
+}
+
+__device__ __forceinline__ int code_of(float x) {  // x already divided by the scale
+    const float r = rintf(x);
+    return (int)fminf(fmaxf(r, -127.f), 127.f);
+}
+
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, const T *xk, const T *xv, int64_t k_stride, int64_t v_stride) {
+    constexpr int DP = 64 * VEC, PITCH = DP + 16;
+    __shared__ uint32_t largest[4][4];                       // [wave][16 tokens]
+    __shared__ __align__(16) uint8_t tile[KV_PAGE * PITCH];  // key codes by token
+    const int tid = threadIdx.x, lane = tid & 63, g = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int head = blockIdx.y;
+    const bool is_v = blockIdx.z;
+    int seq, local, begin, n, first, len;
+    if (!find_item(b.n_seqs, (int)blockIdx.x, [&](int s) { int x, y, z, w; return pages_touched(b, s, true, x, y, z, w); }, seq, local)) return;
+    pages_touched(b, seq, true, begin, n, first, len);
+    const int pi = max(first, 0) / KV_PAGE + local;
+    const int64_t phys = b.pages[(int64_t)seq * b.max_pages + pi];
+    if (phys < 0 || phys >= c.n_pages) return;
+    const int t_lo = max(first - pi * KV_PAGE, 0), t_hi = min(len - pi * KV_PAGE, KV_PAGE);  // the page's new tokens
+    const T *src = is_v ? xv : xk;
+    const int64_t stride = is_v ? v_stride : k_stride;
+    const int64_t row0 = (int64_t)begin + (pi * KV_PAGE - first);  // row of the page's token 0 (may lie before the sequence)
+
+    float x[16][VEC];
+    const bool live = lane * VEC < c.head_dim;
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+        const int t = 16 * (j / 4) + 4 * g + j % 4;
+#pragma unroll
+        for (int v = 0; v < VEC; v++) x[j][v] = 0.f;
+        if (t >= t_lo && t < t_hi) {
+            const T *p = src + (row0 + t) * stride + (int64_t)head * c.head_dim + lane * VEC;
+#pragma unroll
+            for (int v = 0; v < VEC; v++)
+                if (live && lane * VEC + v < c.head_dim) x[j][v] = to_f32(p[v]);
+        }
+    }
+    const int64_t at = (phys * c.kv_heads + head);
+    float *scales = (is_v ? c.vs : c.ks) + at * c.per;
+    uint8_t *codes = (is_v ? c.v : c.k) + at * (KV_PAGE * DP);
+    const int going_on = t_lo % c.block ? t_lo / c.block : -1;  // the block that holds older tokens
+    const float old = going_on >= 0 ? scales[going_on] : 0.f;
+#pragma unroll
+    for (int m = 0; m < 4; m++) {
+        uint32_t big = 0;  // magnitudes as bit patterns: ordered like the numbers, infinity and NaN above all
+#pragma unroll
+        for (int j = 4 * m; j < 4 * m + 4; j++)
+#pragma unroll
+            for (int v = 0; v < VEC; v++) big = max(big, __float_as_uint(x[j][v]) & 0x7fffffffu);
+        big = wave_umax(big);
+        if (lane == 0) largest[g][m] = big;
+    }
+    __syncthreads();
+    float s[4], grown = 0.f;  // scale of the block that 16 tokens belong to; old scale / new scale where older codes move
+    bool moves = false;
+    {
+        uint32_t mx[4];
+#pragma unroll
+        for (int m = 0; m < 4; m++) mx[m] = max(max(largest[0][m], largest[1][m]), max(largest[2][m], largest[3][m]));
+        if (c.block >= 32) { mx[0] = mx[1] = max(mx[0], mx[1]); mx[2] = mx[3] = max(mx[2], mx[3]); }
+        if (c.block >= 64) { mx[0] = mx[1] = mx[2] = mx[3] = max(mx[0], mx[2]); }
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            s[m] = mx[m] >= 0x7f800000u ? __builtin_nanf("") : __uint_as_float(mx[m]) * PER127;
+            if (16 * m / c.block == going_on) {
+                if (s[m] <= old || old != old) s[m] = old;
+                else if (s[m] > old) { grown = old / s[m]; moves = true; }
+            }
+        }
+    }
+    const int moved_lo = moves ? going_on * c.block : t_lo;  // tokens moved_lo .. t_lo - 1 get new codes too
+    if (tid < c.per && tid >= t_lo / c.block && tid <= (t_hi - 1) / c.block) {
+        const int m = tid * c.block / 16;
+        scales[tid] = m < 2 ? (m == 0 ? s[0] : s[1]) : (m == 2 ? s[2] : s[3]);
+    }
+
+    int q[16][VEC];
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+#pragma unroll
+        for (int v = 0; v < VEC; v++) q[j][v] = s[j / 4] > 0.f ? code_of(x[j][v] / s[j / 4]) + 128 : 128;
+
+    if (is_v) {
+        bool any = false, all = true;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int t = 16 * (j / 4) + 4 * g + j % 4;
+            any |= t >= moved_lo && t < t_hi;
+            all &= t >= t_lo && t < t_hi;
+        }
+        if (!any) return;
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+            const int d = lane * VEC + v;
+            if (d >= c.head_dim) continue;
+            uint4 *piece = (uint4 *)(codes + (((d / 16) * 4 + g) * 16 + d % 16) * 16);
+            uint32_t w[4];
+            if (!all) *(uint4 *)w = *piece;
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+                uint32_t r = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int t = 16 * m + 4 * g + i;
+                    uint32_t byte = (uint32_t)q[4 * m + i][v];
+                    if (!all && !(t >= t_lo && t < t_hi)) {
+                        byte = w[m] >> (8 * i) & 0xff;
+                        if (t >= moved_lo && t < t_lo) byte = (uint32_t)(code_of((float)((int)byte - 128) * grown) + 128);
+                    }
+                    r |= byte << (8 * i);
+                }
+                w[m] = r;
+            }
+            *piece = *(uint4 *)w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+        const int t = 16 * (j / 4) + 4 * g + j % 4;
+#pragma unroll
+        for (int v = 0; v < VEC; v++) tile[t * PITCH + lane * VEC + v] = (uint8_t)q[j][v];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < VEC; e++) {  // pieces (64 dimensions e, 16 of them, token), token fastest
+        const int t = tid & 63, p = tid / 64;
+        uint4 *piece = (uint4 *)(codes + (((t / 16 * VEC + e) * 4 + p) * 16 + t % 16) * 16);
+        if (t >= t_lo && t < t_hi) {
+            *piece = *(const uint4 *)(tile + t * PITCH + e * 64 + p * 16);
+        } else if (t >= moved_lo && t < t_lo) {
+            uint32_t w[4];
+            *(uint4 *)w = *piece;
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+                uint32_t r = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) r |= (uint32_t)(code_of((float)((int)(w[m] >> (8 * i) & 0xff) - 128) * grown) + 128) << (8 * i);
+                w[m] = r;
+            }
+            *piece = *(uint4 *)w;
+        }
+    }
+}
+
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void kv_read_kernel(DevKv c, DevBatch b, T *yk, T *yv, int64_t k_stride, int64_t v_stride) {
+    constexpr int DP = 64 * VEC, PITCH = DP + 16;
+    constexpr int OUT = 16 / (int)sizeof(T);  // values of a 16-byte store
+    __shared__ __align__(16) uint8_t tile[KV_PAGE * PITCH];  // codes by token
+    const int tid = threadIdx.x, head = blockIdx.y;
+    const bool is_v = blockIdx.z;
+    int seq, local, begin, n, first, len;
+    if (!find_item(b.n_seqs, (int)blockIdx.x, [&](int s) { int x, y, z, w; return pages_touched(b, s, false, x, y, z, w); }, seq, local)) return;
+    pages_touched(b, seq, false, begin, n, first, len);
+    const int pi = max(first, 0) / KV_PAGE + local;
+    int64_t phys = pi < b.max_pages ? b.pages[(int64_t)seq * b.max_pages + pi] : -1;
+    const bool bad = phys < 0 || phys >= c.n_pages;  // such a page's tokens read as NaN
+    if (bad) phys = 0;
+    const int t_lo = max(first - pi * KV_PAGE, 0), t_hi = min(len - pi * KV_PAGE, KV_PAGE);
+    T *dst = is_v ? yv : yk;
+    const int64_t stride = is_v ? v_stride : k_stride;
+    const int64_t row0 = (int64_t)begin + (pi * KV_PAGE - first);
+    const int64_t at = phys * c.kv_heads + head;
+    const float *scales = (is_v ? c.vs : c.ks) + at * c.per;
+    const uint8_t *codes = (is_v ? c.v : c.k) + at * (KV_PAGE * DP);
+    float s[4];
+#pragma unroll
+    for (int m = 0; m < 4; m++) s[m] = bad ? __builtin_nanf("") : scales[16 * m / c.block];
+#pragma unroll
+    for (int e = 0; e < VEC; e++) {
+        const int i = e * 256 + tid;  // piece in memory order
+        const uint4 w = *(const uint4 *)(codes + (int64_t)i * 16);
+        if (!is_v) {
+            const int t = i / (64 * VEC) * 16 + i % 16, d = i % (64 * VEC) / 64 * 64 + i % 64 / 16 * 16;
+            *(uint4 *)(tile + t * PITCH + d) = w;
+        } else {
+            const int d = i / 64 * 16 + i % 16, g = i % 64 / 16;
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 16; j++) tile[(16 * (j / 4) + 4 * g + j % 4) * PITCH + d] = (uint8_t)(ws[j / 4] >> (8 * (j % 4)));
+        }
+    }
+    __syncthreads();
+    const int per_row = c.head_dim / OUT;
+    const int step_t = 256 / per_row, step_c = 256 % per_row;
+    int t = t_lo + tid / per_row, p = tid % per_row;
+    while (t < t_hi) {
+        const float sc = t < 32 ? (t < 16 ? s[0] : s[1]) : (t < 48 ? s[2] : s[3]);
+        const uint32_t *w = (const uint32_t *)(tile + t * PITCH + p * OUT);
+        T out[OUT] __attribute__((aligned(16)));
+#pragma unroll
+        for (int i = 0; i < OUT; i++) out[i] = (T)((float)((int)(w[i / 4] >> (8 * (i % 4)) & 0xff) - 128) * sc);
+        *(uint4 *)(dst + (row0 + t) * stride + (int64_t)head * c.head_dim + p * OUT) = *(const uint4 *)out;
+        t += step_t;
+        p += step_c;
+        if (p >= per_row) { p -= per_row; t++; }
+    }
+}
+
+template <class T>
+hipError_t write_t(const DevKv &c, const DevBatch &b, const void *k, const void *v, int64_t ks, int64_t vs, dim3 grid, hipStream_t s) {
+    switch (c.dp / 64) {
+    case 1: kv_write_kernel<T, 1><<<grid, 256, 0, s>>>(c, b, (const T *)k, (const T *)v, ks, vs); break;
+    case 2: kv_write_kernel<T, 2><<<grid, 256, 0, s>>>(c, b, (const T *)k, (const T *)v, ks, vs); break;
+    case 3: kv_write_kernel<T, 3><<<grid, 256, 0, s>>>(c, b, (const T *)k, (const T *)v, ks, vs); break;
+    default: kv_write_kernel<T, 4><<<grid, 256, 0, s>>>(c, b, (const T *)k, (const T *)v, ks, vs); break;
+    }
+    return hipGetLastError();
+}
+
+template <class T>
+hipError_t read_t(const DevKv &c, const DevBatch &b, void *k, void *v, int64_t ks, int64_t vs, dim3 grid, hipStream_t s) {
+    switch (c.dp / 64) {
+    case 1: kv_read_kernel<T, 1><<<grid, 256, 0, s>>>(c, b, (T *)k, (T *)v, ks, vs); break;
+    case 2: kv_read_kernel<T, 2><<<grid, 256, 0, s>>>(c, b, (T *)k, (T *)v, ks, vs); break;
+    case 3: kv_read_kernel<T, 3><<<grid, 256, 0, s>>>(c, b, (T *)k, (T *)v, ks, vs); break;
+    default: kv_read_kernel<T, 4><<<grid, 256, 0, s>>>(c, b, (T *)k, (T *)v, ks, vs); break;
+    }
+    return hipGetLastError();
+}
+
+// at most this many (sequence, page) pairs: every one holds a row, and a sequence's rows touch ceil(n / 64) + 1 pages at most
+unsigned page_items(const DevBatch &b) {
+    const int64_t most = b.n_rows / KV_PAGE + 2 * (int64_t)b.n_seqs;
+    return (unsigned)(most < b.n_rows ? most : b.n_rows);
+}
+
+}  // namespace
+
+hipError_t launch_kv_write(const DevKv &c, const DevBatch &b, int type, const void *k, const void *v, int64_t k_stride,
+                           int64_t v_stride, hipStream_t s) {
+    const dim3 grid(page_items(b), (unsigned)c.kv_heads, 2);
+    if (type == T_F32) return write_t<float>(c, b, k, v, k_stride, v_stride, grid, s);
+    if (type == T_F16) return write_t<_Float16>(c, b, k, v, k_stride, v_stride, grid, s);
+    return write_t<__bf16>(c, b, k, v, k_stride, v_stride, grid, s);
+}
+
+hipError_t launch_kv_read(const DevKv &c, const DevBatch &b, int type, void *k, void *v, int64_t k_stride, int64_t v_stride,
+                          hipStream_t s) {
+    const dim3 grid(page_items(b), (unsigned)c.kv_heads, 2);
+    if (type == T_F32) return read_t<float>(c, b, k, v, k_stride, v_stride, grid, s);
+    if (type == T_F16) return read_t<_Float16>(c, b, k, v, k_stride, v_stride, grid, s);
+    return read_t<__bf16>(c, b, k, v, k_stride, v_stride, grid, s);
+}
+
+}  // namespace miqmm

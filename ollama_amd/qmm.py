@@ -29,6 +29,9 @@ PRODUCE_NONE, PRODUCE_RMSNORM, PRODUCE_SWIGLU = 0, 1, 2
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_HIP, ERR_NOMEM, ERR_NODEVICE = 0, -1, -2, -3, -4, -5
 
 NOALLOC_SCRATCH_BYTES = 16 << 20  # MI_QMM_NOALLOC_SCRATCH_BYTES
+STREAM_LEGACY = 1  # hipStreamLegacy: HIP's default stream as an argument of Context.set_stream
+ROPE_HALVES, ROPE_ADJACENT = 0, 1  # which values a rotation pairs (MI_QMM_ROPE_*)
+KV_PAGE = 64  # tokens of a cache page (MI_QMM_KV_PAGE)
 
 EXPORTS = [
     "mi_qmm_block_size", "mi_qmm_type_size", "mi_qmm_row_size", "mi_qmm_vec_dot_type",
@@ -42,6 +45,8 @@ EXPORTS = [
     "mi_qmm_gguf_tensor_data", "mi_qmm_gguf_find_kv", "mi_qmm_gguf_kv", "mi_qmm_gguf_kv_int", "mi_qmm_gguf_kv_uint",
     "mi_qmm_gguf_kv_float", "mi_qmm_gguf_kv_bool", "mi_qmm_gguf_kv_string", "mi_qmm_gguf_upload",
     "mi_qmm_last_error", "mi_qmm_version", "mi_qmm_device_info",
+    "mi_qmm_qk_norm_rope", "mi_qmm_rope_freqs", "mi_qmm_kv_bytes", "mi_qmm_kv_create", "mi_qmm_kv_free", "mi_qmm_kv_write",
+    "mi_qmm_kv_read", "mi_qmm_attention",
 ]
 
 
@@ -131,6 +136,17 @@ def lib() -> ctypes.CDLL:
     L.mi_qmm_gguf_kv_bool.restype = ci; L.mi_qmm_gguf_kv_bool.argtypes = [vp, i64, i64, P(ci)]
     L.mi_qmm_gguf_kv_string.restype = ci; L.mi_qmm_gguf_kv_string.argtypes = [vp, i64, i64, P(vp), P(i64)]
     L.mi_qmm_gguf_upload.restype = ci; L.mi_qmm_gguf_upload.argtypes = [vp, vp, i64, P(vp)]
+    cd, P_ = ctypes.c_double, ctypes.POINTER
+    L.mi_qmm_rope_freqs.restype = ci
+    L.mi_qmm_rope_freqs.argtypes = [ci, cd, cd, cd, cd, cd, cd, ci, vp, vp, P_(ctypes.c_float)]
+    L.mi_qmm_qk_norm_rope.restype = ci
+    L.mi_qmm_qk_norm_rope.argtypes = [vp, vp, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, ci]
+    L.mi_qmm_kv_bytes.restype = i64; L.mi_qmm_kv_bytes.argtypes = [i64, ci, ci, ci]
+    L.mi_qmm_kv_create.restype = ci; L.mi_qmm_kv_create.argtypes = [vp, i64, ci, ci, ci, vp, P_(vp)]
+    L.mi_qmm_kv_free.restype = None; L.mi_qmm_kv_free.argtypes = [vp]
+    L.mi_qmm_kv_write.restype = ci; L.mi_qmm_kv_write.argtypes = [vp, vp, vp, ci, vp, i64, vp, i64, i64, ci]
+    L.mi_qmm_kv_read.restype = ci; L.mi_qmm_kv_read.argtypes = [vp, vp, vp, ci, vp, i64, vp, i64, i64, ci]
+    L.mi_qmm_attention.restype = ci; L.mi_qmm_attention.argtypes = [vp, vp, vp, vp, vp, i64, vp, i64, i64, ci]
     L.mi_qmm_last_error.restype = ctypes.c_char_p; L.mi_qmm_last_error.argtypes = []
     L.mi_qmm_version.restype = ctypes.c_char_p; L.mi_qmm_version.argtypes = []
     L.mi_qmm_device_info.restype = ci
@@ -218,6 +234,110 @@ class Act:
             self.free()
         except Exception:
             pass
+
+
+class _QKHeads(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int), ("n_heads", ctypes.c_int), ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("n_rot", ctypes.c_int), ("pairing", ctypes.c_int), ("eps", ctypes.c_float), ("mscale", ctypes.c_float),
+                ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("freqs", ctypes.c_void_p)]
+
+
+class _Batch(ctypes.Structure):
+    _fields_ = [("n_seqs", ctypes.c_int), ("max_pages", ctypes.c_int), ("row_start", ctypes.c_void_p),
+                ("kv_len", ctypes.c_void_p), ("pages", ctypes.c_void_p)]
+
+
+class _Attn(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int), ("n_heads", ctypes.c_int), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+                ("causal", ctypes.c_int), ("window", ctypes.c_int), ("sinks", ctypes.c_void_p)]
+
+
+class QKHeads:
+    """The heads of qk_norm_rope (mi_qmm_qk_heads): types and counts, the rotation, the norm weights.  The pointers are
+    device addresses (or host ones for a call with host arrays) that stay valid as long as it is used."""
+
+    def __init__(self, ggml_type: int, n_heads: int, n_kv_heads: int, head_dim: int, freqs_ptr, n_rot: int,
+                 pairing: int = ROPE_HALVES, mscale: float = 1.0, q_weight=None, k_weight=None, eps: float = 0.0):
+        self._s = _QKHeads(ggml_type, n_heads, n_kv_heads, head_dim, n_rot, pairing, eps, mscale, q_weight, k_weight, freqs_ptr)
+        self._p = ctypes.addressof(self._s)
+        self.q_row, self.k_row = n_heads * head_dim, n_kv_heads * head_dim
+
+
+class Batch:
+    """The sequences of a step (mi_qmm_batch): device addresses of row_start int32 [n_seqs + 1], kv_len int32 [n_seqs]
+    and pages int32 [n_seqs][max_pages]; or, from numpy arrays, host ones (Batch.of)."""
+
+    def __init__(self, n_seqs: int, max_pages: int, row_start_ptr, kv_len_ptr, pages_ptr):
+        self._s = _Batch(n_seqs, max_pages, row_start_ptr, kv_len_ptr, pages_ptr)
+        self._p = ctypes.addressof(self._s)
+        self._keep = None
+
+    @classmethod
+    def of(cls, row_start, kv_len, pages) -> "Batch":
+        row_start, kv_len = np.ascontiguousarray(row_start, np.int32), np.ascontiguousarray(kv_len, np.int32)
+        pages = np.ascontiguousarray(pages, np.int32)
+        if pages.ndim != 2 or row_start.shape != (pages.shape[0] + 1,) or kv_len.shape != (pages.shape[0],):
+            raise ValueError(f"row_start {row_start.shape}, kv_len {kv_len.shape} and pages {pages.shape} do not fit together")
+        b = cls(pages.shape[0], pages.shape[1], row_start.ctypes.data, kv_len.ctypes.data, pages.ctypes.data)
+        b._keep = (row_start, kv_len, pages)
+        return b
+
+
+class Attention:
+    """How rows attend (mi_qmm_attn): type, query heads, scale, and what limits or caps the scores."""
+
+    def __init__(self, ggml_type: int, n_heads: int, scale: float, window: int = 0, softcap: float = 0.0, sinks=None,
+                 causal: bool = True):
+        self._s = _Attn(ggml_type, n_heads, scale, softcap, 1 if causal else 0, window, sinks)
+        self._p = ctypes.addressof(self._s)
+        self.n_heads = n_heads
+
+
+class KVCache:
+    """A key/value cache in 8 bits (mi_qmm_kv)."""
+
+    def __init__(self, handle, n_pages: int, n_kv_heads: int, head_dim: int, block: int):
+        self._h = handle
+        self.n_pages, self.n_kv_heads, self.head_dim, self.block = n_pages, n_kv_heads, head_dim, block
+        self.row = n_kv_heads * head_dim
+
+    def free(self):
+        if self._h:
+            lib().mi_qmm_kv_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def kv_bytes(n_pages: int, n_kv_heads: int, head_dim: int, block: int) -> int:
+    """device bytes of a cache; -1 where there is no such cache"""
+    return int(lib().mi_qmm_kv_bytes(n_pages, n_kv_heads, head_dim, block))
+
+
+def rope_freqs(n_rot: int, base: float, freq_scale: float = 1.0, ext_factor: float = 0.0, attn_factor: float = 1.0,
+               beta_fast: float = 32.0, beta_slow: float = 1.0, n_ctx_orig: int = 0, factors=None):
+    """(radians per position as float64 [n_rot / 2], mscale) for QKHeads: plain, linear, YaRN or per-frequency scaling"""
+    freqs, mscale = np.empty(max(n_rot, 0) // 2, np.float64), ctypes.c_float()
+    if factors is not None:
+        factors = np.ascontiguousarray(factors, np.float32)
+        if factors.shape != freqs.shape:
+            raise ValueError(f"factors {factors.shape}, want {freqs.shape}")
+    _check(lib().mi_qmm_rope_freqs(n_rot, base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow, n_ctx_orig,
+                                   None if factors is None else factors.ctypes.data, freqs.ctypes.data, ctypes.byref(mscale)))
+    return freqs, mscale.value
+
+
+_VALUES = {np.dtype(np.float32): F32, np.dtype(np.float16): F16}  # numpy has no bfloat16: BF16 goes through the _device calls
+
+
+def _value_type(a: np.ndarray) -> int:
+    if a.dtype not in _VALUES:
+        raise TypeError(f"values must be float32 or float16, got {a.dtype}")
+    return _VALUES[a.dtype]
 
 
 class Context:
@@ -344,6 +464,93 @@ class Context:
         """while frozen, a call that would have to grow the ctx's scratch raises instead of reallocating
         (captured HIP graphs keep the old addresses)."""
         _check(lib().mi_qmm_scratch_freeze(self._h, 1 if frozen else 0))
+
+    # ---- rotation, cache, attention ---------------------------------------------------------------
+    def qk_norm_rope(self, q: np.ndarray, k, pos, freqs, pairing: int = ROPE_HALVES, mscale: float = 1.0, q_weight=None,
+                     k_weight=None, eps: float = 0.0):
+        """norms per head and rotation of q [n, heads, dim] and k [n, kv_heads, dim] (or None) at positions pos [n];
+        freqs float64 [n_rot / 2] (rope_freqs); host arrays, returns new ones"""
+        q, pos, freqs = np.ascontiguousarray(q), np.ascontiguousarray(pos, np.int32), np.ascontiguousarray(freqs, np.float64)
+        t = _value_type(q)
+        k = None if k is None else np.ascontiguousarray(k)
+        if q.ndim != 3 or pos.shape != q.shape[:1] or (k is not None and (k.ndim != 3 or k.dtype != q.dtype or k.shape[::2] != q.shape[::2])):
+            raise ValueError(f"q {q.shape}, k {None if k is None else k.shape} and pos {pos.shape} do not fit together")
+        n, heads, dim = q.shape
+        ws = [None if w is None else np.ascontiguousarray(w, np.float32) for w in (q_weight, k_weight)]
+        if any(w is not None and w.shape != (dim,) for w in ws):
+            raise ValueError(f"norm weights must hold {dim} values")
+        h = QKHeads(t, heads, 0 if k is None else k.shape[1], dim, freqs.ctypes.data, 2 * freqs.size, pairing, mscale,
+                    *[None if w is None else w.ctypes.data for w in ws], eps)
+        qo, ko = np.empty_like(q), None if k is None else np.empty_like(k)
+        _check(lib().mi_qmm_qk_norm_rope(self._h, h._p, _ptr(q), h.q_row, _ptr(k), h.k_row, _ptr(pos), n, _ptr(qo), h.q_row,
+                                         _ptr(ko), h.k_row, HOST))
+        return qo, ko
+
+    def qk_norm_rope_device(self, heads: QKHeads, q_ptr, k_ptr, pos_ptr, n: int, q_out_ptr, k_out_ptr, q_stride=None,
+                            k_stride=None, q_out_stride=None, k_out_stride=None):
+        """device pointers; strides in values from row to row (None: rows without gaps)"""
+        q, k = heads.q_row, heads.k_row
+        rc = lib().mi_qmm_qk_norm_rope(self._h, heads._p, q_ptr, q_stride or q, k_ptr, k_stride or k, pos_ptr, n, q_out_ptr,
+                                       q_out_stride or q, k_out_ptr, k_out_stride or k, DEVICE)
+        if rc:
+            _check(rc)
+
+    def kv_create(self, n_pages: int, n_kv_heads: int, head_dim: int, block: int = 64, memory=None) -> KVCache:
+        """a cache of n_pages pages of 64 tokens, a scale per `block` tokens and head; memory: device address of
+        kv_bytes() bytes that outlives the cache, or None (the library allocates)"""
+        h = ctypes.c_void_p()
+        _check(lib().mi_qmm_kv_create(self._h, n_pages, n_kv_heads, head_dim, block, memory, ctypes.byref(h)))
+        return KVCache(h, n_pages, n_kv_heads, head_dim, block)
+
+    def _kv_shape(self, kv: KVCache, a: np.ndarray, name: str):
+        if a.ndim != 3 or a.shape[1:] != (kv.n_kv_heads, kv.head_dim):
+            raise ValueError(f"{name} {a.shape}, want [n, {kv.n_kv_heads}, {kv.head_dim}]")
+
+    def kv_write(self, kv: KVCache, batch: Batch, k: np.ndarray, v: np.ndarray):
+        """k, v [n, kv_heads, dim] (host) into the cache; batch from Batch.of"""
+        k, v = np.ascontiguousarray(k), np.ascontiguousarray(v)
+        self._kv_shape(kv, k, "k")
+        if v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError(f"k {k.shape} {k.dtype} and v {v.shape} {v.dtype} differ")
+        _check(lib().mi_qmm_kv_write(self._h, kv._h, batch._p, _value_type(k), _ptr(k), kv.row, _ptr(v), kv.row, k.shape[0], HOST))
+
+    def kv_read(self, kv: KVCache, batch: Batch, n: int, dtype=np.float32):
+        """(k, v) [n, kv_heads, dim] of the batch's rows (host); rows of no sequence are zeros"""
+        k = np.zeros((n, kv.n_kv_heads, kv.head_dim), dtype)
+        v = np.zeros_like(k)
+        _check(lib().mi_qmm_kv_read(self._h, kv._h, batch._p, _value_type(k), _ptr(k), kv.row, _ptr(v), kv.row, n, HOST))
+        return k, v
+
+    def attention(self, kv: KVCache, batch: Batch, q: np.ndarray, scale: float, window: int = 0, softcap: float = 0.0,
+                  sinks=None, causal: bool = True) -> np.ndarray:
+        """attention of q [n, heads, dim] (host) over the cache; rows of no sequence are zeros"""
+        q = np.ascontiguousarray(q)
+        if q.ndim != 3 or q.shape[2] != kv.head_dim:
+            raise ValueError(f"q {q.shape}, the cache has heads of {kv.head_dim}")
+        if sinks is not None:
+            sinks = np.ascontiguousarray(sinks, np.float32)
+            if sinks.shape != (q.shape[1],):
+                raise ValueError(f"sinks {sinks.shape}, q has {q.shape[1]} heads")
+        how = Attention(_value_type(q), q.shape[1], scale, window, softcap, None if sinks is None else sinks.ctypes.data, causal)
+        out, row = np.zeros_like(q), q.shape[1] * q.shape[2]
+        _check(lib().mi_qmm_attention(self._h, kv._h, batch._p, how._p, _ptr(q), row, _ptr(out), row, q.shape[0], HOST))
+        return out
+
+    def kv_write_device(self, kv: KVCache, batch: Batch, ggml_type: int, k_ptr, v_ptr, n: int, k_stride=None, v_stride=None):
+        rc = lib().mi_qmm_kv_write(self._h, kv._h, batch._p, ggml_type, k_ptr, k_stride or kv.row, v_ptr, v_stride or kv.row, n, DEVICE)
+        if rc:
+            _check(rc)
+
+    def kv_read_device(self, kv: KVCache, batch: Batch, ggml_type: int, k_ptr, v_ptr, n: int, k_stride=None, v_stride=None):
+        rc = lib().mi_qmm_kv_read(self._h, kv._h, batch._p, ggml_type, k_ptr, k_stride or kv.row, v_ptr, v_stride or kv.row, n, DEVICE)
+        if rc:
+            _check(rc)
+
+    def attention_device(self, kv: KVCache, batch: Batch, how: Attention, q_ptr, n: int, out_ptr, q_stride=None, out_stride=None):
+        row = how.n_heads * kv.head_dim
+        rc = lib().mi_qmm_attention(self._h, kv._h, batch._p, how._p, q_ptr, q_stride or row, out_ptr, out_stride or row, n, DEVICE)
+        if rc:
+            _check(rc)
 
     # ---- two-phase form -------------------------------------------------------------------------
     def act_create(self, q8_type: int, k: int, n_max: int) -> Act:
