@@ -10,8 +10,12 @@
 //
 // The first product is K Q^T and the second V^T P^T: a lane's scores are then of one row, its maximum and sum are scalars
 // of the lane, and the probabilities are already the second product's operand.
-//   key codes as subnormal halves (code + 128) 2^-24: the accumulators start at -128 2^-24 sum q, which takes the 128 out
-//   value codes: the 128 is subtracted from the halves -- left in, sum p (code + 128) would be hundreds of times the result
+//   key codes of 16-bit calls as subnormal halves (code + 128) 2^-24, one byte permute per pair: the accumulators start at
+//   -128 2^-24 sum q, which takes the 128 out.  The matrix cores align a product by its operands' exponent fields, and a
+//   subnormal's is that of 2^-14: ten bits of the sum are lost, 6e-6 of a score (measured), nothing to 16-bit results but
+//   too much for f32
+//   key codes of f32 calls, and value codes, as the whole numbers themselves: 1024 + byte less 1152, one more instruction
+//   per pair (left in, 128 would make sum p (code + 128) hundreds of times the result)
 //   scales of keys multiply the scores; scales of values the probabilities, against a running power of two so that the
 //   product is at most 1
 #include "internal.h"
@@ -58,11 +62,14 @@ __device__ __forceinline__ half8 widen(uint32_t lo, uint32_t hi) {
     return r.v;
 }
 
-// the same less 128 * 2^-24
+// eight code bytes to the codes as halves: 0x6400 | byte is 1024 + byte
 __device__ __forceinline__ half8 widen_centred(uint32_t lo, uint32_t hi) {
     Halves r, c;
-    r.v = widen(lo, hi);
-    c.u[0] = 0x00800080u;
+    r.u[0] = __builtin_amdgcn_perm(0x64646464u, lo, 0x04010400u);
+    r.u[1] = __builtin_amdgcn_perm(0x64646464u, lo, 0x04030402u);
+    r.u[2] = __builtin_amdgcn_perm(0x64646464u, hi, 0x04010400u);
+    r.u[3] = __builtin_amdgcn_perm(0x64646464u, hi, 0x04030402u);
+    c.u[0] = 0x64806480u;  // 1152
 #pragma unroll
     for (int i = 0; i < 4; i++) r.h[i] = r.h[i] - c.h[0];
     return r.v;
@@ -91,7 +98,8 @@ constexpr int ROWS = 16;
 
 template <class T, int NC, bool CAP>
 __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
-    constexpr bool HILO = sizeof(T) == 4;
+    constexpr bool HILO = sizeof(T) == 4;                // queries in two halves
+    constexpr bool PHILO = !__is_same(T, __bf16);  // probabilities in two halves
     constexpr int DP = 64 * NC;
     using V4 = typename Vec4<T>::type;
     __shared__ float part_o[4][ROWS][64 + 4];
@@ -152,15 +160,15 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
             }
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
-        minus_bias = sum * (-128.f * 0x1p-24f);
-        score_scale = a.scale * 0x1p24f * pow2(-e) * (CAP ? 1.f : LOG2E);
+        minus_bias = HILO ? 0.f : sum * (-128.f * 0x1p-24f);
+        score_scale = a.scale * (HILO ? 1.f : 0x1p24f) * pow2(-e) * (CAP ? 1.f : LOG2E);
     }
 
     float4v acc[4 * NC];
 #pragma unroll
     for (int i = 0; i < 4 * NC; i++) acc[i] = float4v{0.f, 0.f, 0.f, 0.f};
     float m = MINUS_INF, l = 0.f;
-    float ref = 0x1p-100f;  // values are accumulated in units of ref * 2^-15 * 2^-24
+    float ref = 0x1p-100f;  // values are accumulated in units of ref * 2^-15
 
     int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
     if (a.splits > 1) {
@@ -195,7 +203,8 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
             float4v s = {minus_bias, minus_bias, minus_bias, minus_bias};
 #pragma unroll
             for (int c = 0; c < NC; c++) {
-                const half8 k0 = widen(kc[t][c].x, kc[t][c].y), k1 = widen(kc[t][c].z, kc[t][c].w);
+                const half8 k0 = HILO ? widen_centred(kc[t][c].x, kc[t][c].y) : widen(kc[t][c].x, kc[t][c].y);
+                const half8 k1 = HILO ? widen_centred(kc[t][c].z, kc[t][c].w) : widen(kc[t][c].z, kc[t][c].w);
                 s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[2 * c].v, s, 0, 0, 0);
                 s = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[2 * c + 1].v, s, 0, 0, 0);
                 if (HILO) {
@@ -248,14 +257,14 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
             const float y = z[i] == MINUS_INF ? 0.f : p * (vs[i / 4] * (0x1p15f / ref));
             const _Float16 h = (_Float16)y;
             ph[i / 8].v[i % 8] = h;
-            if (HILO) pl[i / 8].v[i % 8] = (_Float16)(y - (float)h);
+            if (PHILO) pl[i / 8].v[i % 8] = (_Float16)(y - (float)h);
         }
 #pragma unroll
         for (int d = 0; d < 4 * NC; d++) {
             const half8 v0 = widen_centred(vc[d].x, vc[d].y), v1 = widen_centred(vc[d].z, vc[d].w);
             acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[0].v, acc[d], 0, 0, 0);
             acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[1].v, acc[d], 0, 0, 0);
-            if (HILO) {
+            if (PHILO) {
                 acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[0].v, acc[d], 0, 0, 0);
                 acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[1].v, acc[d], 0, 0, 0);
             }
@@ -276,7 +285,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
     };
     float top, base, sum;
     joined(r, top, base, sum);
-    const float weight = __builtin_amdgcn_exp2f(m - base) * (ref * (0x1p-15f * 0x1p24f));
+    const float weight = __builtin_amdgcn_exp2f(m - base) * (ref * 0x1p-15f);
 
     const int o_row = tid / 16, o_d = tid % 16 * 4;  // what this thread writes of 64 dimensions
     const bool writes = row0 + o_row < rows;
