@@ -321,7 +321,7 @@ int mi_qmm_mulmat_id_produced(mi_qmm_ctx *ctx, const mi_qmm_weight *w, int n_exp
  *      Rotation, cache and attention take activations of type MI_QMM_TYPE_F32, _F16 or _BF16 (the products' own are f32);
  *      sums, softmax statistics and norms are fp32 and every result is rounded once.  Row pointers are 16-byte aligned
  *      and row strides (elements from one row to the next, at least a row's values) whole 16-byte pieces in bytes;
- *      head_dim is a multiple of 8 up to 256; anything else is MI_QMM_ERR_INVALID or _UNSUPPORTED.  `location` covers
+ *      head_dim is a multiple of 8 up to 256; a call has at most 2^22 rows, attention 2^27 rows times heads; anything else is MI_QMM_ERR_INVALID or _UNSUPPORTED.  `location` covers
  *      every pointer of a call, those inside the structs included; a cache is always device memory. */
 
 /* Norms of queries and keys for each head and the rotation by position, in one pass:

@@ -29,6 +29,10 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 
+typedef float float16v __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(1))) const void glb_ptr_t;
+typedef __attribute__((address_space(3))) void lds_ptr_t;
+
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float MINUS_INF = -__builtin_inff();
 
@@ -42,8 +46,9 @@ struct AttnLaunch {
     float scale, softcap;
     int causal, window;
     const float *sinks;
-    float *part;  // [item][kv head][split]: ROWS x dp numerators, ROWS maxima, ROWS sums
-    int splits;
+    float *part;  // [item][kv head][split]: R x dp numerators, R maxima, R sums (R rows per tile)
+    int splits, items;
+    int most, least;  // sequences of least..most (token, head) rows per key/value head are this launch's
 };
 
 union Halves {
@@ -75,19 +80,42 @@ __device__ __forceinline__ half8 widen_centred(uint32_t lo, uint32_t hi) {
     return r.v;
 }
 
+// x as the fp32 number that it is: rounding a product to half straight from its operands (one instruction) can give
+// another half than rounding the fp32 product, and the second half would then be the remainder of the wrong one
+__device__ __forceinline__ float settled(float x) {
+    asm("" : "+v"(x));
+    return x;
+}
+
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
 __device__ __forceinline__ int exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 0xff) - 127; }
 
-// what the rows of one tile see, and where the tile lies
-struct TileRows {
-    int begin, n, len, first;  // the sequence: first row, rows, tokens, position of its first row
-    int row0, rows;            // first (token, head) row of the tile, and one past the sequence's last
-};
+// tiles of R rows that this launch has in sequence s
+template <int R>
+__device__ __forceinline__ int tiles_of(const AttnLaunch &a, int s) {
+    int begin;
+    const int rows = seq_rows(a.b, s, begin) * a.group;
+    return rows >= a.least && rows <= a.most ? (rows + R - 1) / R : 0;
+}
 
 __device__ __forceinline__ void visible(const AttnLaunch &a, int pos, int len, int &lo, int &hi) {
     lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
     hi = a.causal ? min(pos + 1, len) : len;
     hi = max(hi, 0);
+}
+
+// Scales that are no numbers (a poisoned block, a page that there is not) are taken out of a page's work -- masked tokens of
+// such a block would turn into NaN -- and make NaN of the sum of a row (lo .. hi - 1) that sees one of the block's tokens.
+__device__ __forceinline__ void take_out_nan(float (&ks)[4], float (&vs)[4], int j0, int lo, int hi, float &l) {
+    const float all = ks[0] + ks[1] + ks[2] + ks[3] + vs[0] + vs[1] + vs[2] + vs[3];
+    if (all - all == 0.f) return;
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        const float both = ks[t] + vs[t];
+        if (both - both == 0.f) continue;
+        ks[t] = vs[t] = 0.f;
+        if (max(lo, j0 + 16 * t) < min(hi, j0 + 16 * t + 16)) l = __builtin_nanf("");
+    }
 }
 
 // ---- 16 rows per workgroup: a step of few tokens --------------------------------------------------------------------
@@ -108,8 +136,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
     const int r = lane % 16, g = lane / 16;
     const int head = blockIdx.y;  // key/value head
     int seq, tile;
-    auto tiles = [&](int s) { int begin; const int n = seq_rows(a.b, s, begin); return (int)(((int64_t)n * a.group + ROWS - 1) / ROWS); };
-    if (!find_item(a.b.n_seqs, (int)blockIdx.x, tiles, seq, tile)) return;
+    if (!find_item(a.b.n_seqs, (int)blockIdx.x, [&](int s) { return tiles_of<ROWS>(a, s); }, seq, tile)) return;
     int begin;
     const int n = seq_rows(a.b, seq, begin), len = a.b.kv_len[seq], first = len - n;
     const int rows = n * a.group, row0 = tile * ROWS;
@@ -197,6 +224,8 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
             ks[t] = bad ? __builtin_nanf("") : a.c.ks[i];
             vs[t] = bad ? __builtin_nanf("") : a.c.vs[i];
         }
+        const int j0 = page * KV_PAGE;
+        take_out_nan(ks, vs, j0, lo, hi, l);
         float z[16];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
@@ -219,7 +248,6 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
                 if (CAP) z[4 * t + i] = a.softcap * LOG2E * tanhf(z[4 * t + i] / a.softcap);
             }
         }
-        const int j0 = page * KV_PAGE;
         if (j0 < lo_max || j0 + KV_PAGE > hi_min) {
 #pragma unroll
             for (int i = 0; i < 16; i++) {
@@ -253,8 +281,8 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
         for (int i = 0; i < 16; i++) {
             const float p = __builtin_amdgcn_exp2f(z[i] - base);
             l += p;
-            // a masked token counts nothing, whatever its scale is
-            const float y = z[i] == MINUS_INF ? 0.f : p * (vs[i / 4] * (0x1p15f / ref));
+            float y = p * (vs[i / 4] * (0x1p15f / ref));
+            if (PHILO) y = settled(y);
             const _Float16 h = (_Float16)y;
             ph[i / 8].v[i % 8] = h;
             if (PHILO) pl[i / 8].v[i % 8] = (_Float16)(y - (float)h);
@@ -339,32 +367,290 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
     }
 }
 
+// ---- 128 rows per workgroup: prompts ----------------------------------------------------------------------------------
+// Bound: the vector ALU beside the matrix cores.  A wave holds 32 rows, the workgroup's four waves share each page of 64
+// tokens through LDS (two buffers, loaded straight into them while the page before is worked on).  Per page and wave of 32
+// rows at a head of 128 the matrix cores have 1024 cycles of work; widening the codes and the softmax of 2048 scores, a
+// quarter-rate exponential each, are about twice that.
+constexpr int TILE = 128;
+
+template <class T, int NC, bool CAP>
+__global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLaunch a) {
+    constexpr bool HILO = sizeof(T) == 4;              // queries in two halves
+    constexpr bool PHILO = !__is_same(T, __bf16);      // probabilities in two halves
+    constexpr int DP = 64 * NC, BYTES = KV_PAGE * DP;  // of a page's keys (and values) of one head
+    using V4 = typename Vec4<T>::type;
+    __shared__ __align__(1024) uint8_t buf[2][2 * BYTES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int r = lane % 32, h = lane / 32;
+    // heads fastest: with eight of them every XCD keeps one head's cache in its L2; later tiles (longer ones) first
+    const int head = blockIdx.x % a.c.kv_heads, item = a.items - 1 - (int)blockIdx.x / a.c.kv_heads;
+    int seq, tile;
+    if (!find_item(a.b.n_seqs, item, [&](int s) { return tiles_of<TILE>(a, s); }, seq, tile)) return;
+    int begin;
+    const int n = seq_rows(a.b, seq, begin), len = a.b.kv_len[seq], first = len - n;
+    const int rows = n * a.group, row0 = tile * TILE, wrow0 = row0 + 32 * wave;
+    const bool valid = wrow0 + r < rows;
+    const int my_t = valid ? (wrow0 + r) / a.group : 0, my_h = valid ? wrow0 + r - my_t * a.group : 0;
+    int lo, hi, lo_min, lo_max, hi_min, hi_max, w_lo_min, w_lo_max, w_hi_min, w_hi_max;
+    visible(a, first + my_t, len, lo, hi);
+    visible(a, first + row0 / a.group, len, lo_min, hi_min);
+    visible(a, first + (min(row0 + TILE, rows) - 1) / a.group, len, lo_max, hi_max);
+    visible(a, first + min(wrow0, rows - 1) / a.group, len, w_lo_min, w_hi_min);
+    visible(a, first + (min(wrow0 + 32, rows) - 1) / a.group, len, w_lo_max, w_hi_max);
+
+    // queries: dimensions 64 c + 16 (2 e + h) + 8 i .. + 7 of row r, as the second operand of step (c, e, i)
+    Halves qh[NC][2][2], ql[HILO ? NC : 1][2][2];
+    float score_scale, minus_bias;
+    {
+        float x[NC][2][16];
+        float big = 0.f;
+        const T *p = (const T *)a.q + (int64_t)(begin + my_t) * a.q_stride + (int64_t)(head * a.group + my_h) * a.c.head_dim;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int d = 64 * c + 16 * (2 * (i / 4) + h) + 4 * (i % 4);
+                V4 y = {};
+                if (valid && d < a.c.head_dim) y = *(const V4 *)(p + d);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    x[c][i / 4][4 * (i % 4) + e] = to_f32(y[e]);
+                    big = fmaxf(big, fabsf(to_f32(y[e])));
+                }
+            }
+        big = fmaxf(big, __shfl_xor(big, 32));
+        const int e = min(max(13 - exponent(big), -100), 100);
+        const float up = a.scale < 0.f ? -pow2(e) : pow2(e);  // the scale's sign goes into the queries
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+                const float y = x[c][i / 16][i % 16] * up;
+                const _Float16 z = (_Float16)y;
+                qh[c][i / 16][i / 8 % 2].v[i % 8] = z;
+                sum += (float)z;
+                if (HILO) ql[HILO ? c : 0][i / 16][i / 8 % 2].v[i % 8] = (_Float16)(y - (float)z);
+            }
+        sum += __shfl_xor(sum, 32);
+        minus_bias = HILO ? 0.f : sum * (-128.f * 0x1p-24f);
+        score_scale = fabsf(a.scale) * (HILO ? 1.f : 0x1p24f) * pow2(-e) * (CAP ? 1.f : LOG2E);
+    }
+
+    float16v acc[2 * NC];
+#pragma unroll
+    for (int d = 0; d < 2 * NC; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
+    float m = MINUS_INF, l = 0.f, ref = 0x1p-100f;
+
+    int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
+    if (a.splits > 1) {
+        const int share = (t1 - t0 + a.splits - 1) / a.splits;
+        t0 = t0 + (int)blockIdx.z * share;
+        t1 = min(t1, t0 + share);
+    }
+    // a page's number, two pages ahead of its use: the number, then its codes and scales, then the work
+    auto page_at = [&](int page) {
+        const int64_t phys = page < t1 && page < a.b.max_pages ? a.b.pages[(int64_t)seq * a.b.max_pages + page] : -1;
+        return phys < a.c.n_pages ? phys : -1;
+    };
+    float ks[4], vs[4];
+    auto fetch = [&](int64_t phys, int b) {
+        const bool bad = phys < 0;  // no such page: whoever sees it gets NaN
+        const int64_t at = (bad ? 0 : phys) * a.c.kv_heads + head;
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+            const int kb = (wave * NC + i) * 1024;
+            __builtin_amdgcn_global_load_lds((glb_ptr_t *)(a.c.k + at * BYTES + kb + lane * 16), (lds_ptr_t *)(buf[b] + kb), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((glb_ptr_t *)(a.c.v + at * BYTES + kb + lane * 16), (lds_ptr_t *)(buf[b] + BYTES + kb), 16, 0, 0);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int64_t i = at * a.c.per + 16 * t / a.c.block;
+            ks[t] = bad ? __builtin_nanf("") : a.c.ks[i];
+            vs[t] = bad ? __builtin_nanf("") : a.c.vs[i];
+        }
+    };
+    int64_t next = page_at(t0);
+    if (t0 < t1) fetch(next, 0);
+    next = page_at(t0 + 1);
+    for (int page = t0; page < t1; page++) {
+        const int b = (page - t0) & 1;
+        const int j0 = page * KV_PAGE;
+        take_out_nan(ks, vs, j0, lo, hi, l);
+        float f[4], w[4];
+        const float vmax = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            f[t] = score_scale * ks[t];
+            if (f[t] == 0.f) f[t] = 1e-30f;  // times a masked token's -inf stays -inf; all else is 0 either way
+            w[t] = vs[t];
+        }
+        __builtin_amdgcn_s_waitcnt((0 & 15) | (7 << 4) | (15 << 8));  // vmcnt(0): this wave's part of the page is in LDS
+        __syncthreads();
+        if (page + 1 < t1) {
+            fetch(next, b ^ 1);
+            next = page_at(page + 2);
+        }
+        if (wrow0 >= rows || j0 >= w_hi_max || j0 + KV_PAGE <= w_lo_min) continue;  // nothing that this wave's rows see
+        const uint8_t *kb = buf[b], *vb = buf[b] + BYTES;
+        float16v s[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[t][i] = minus_bias;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const uint4 x = *(const uint4 *)(kb + (((2 * t + r / 16) * NC + c) * 64 + (2 * e + h) * 16 + r % 16) * 16);
+                    const half8 k0 = HILO ? widen_centred(x.x, x.y) : widen(x.x, x.y);
+                    const half8 k1 = HILO ? widen_centred(x.z, x.w) : widen(x.z, x.w);
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qh[c][e][0].v, s[t], 0, 0, 0);
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[c][e][1].v, s[t], 0, 0, 0);
+                    if (HILO) {
+                        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[HILO ? c : 0][e][0].v, s[t], 0, 0, 0);
+                        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[HILO ? c : 0][e][1].v, s[t], 0, 0, 0);
+                    }
+                }
+        }
+        if (CAP) {
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+                const int t = i / 8;
+                s[i / 16][i % 16] = a.softcap * LOG2E * tanhf(s[i / 16][i % 16] * f[t] / a.softcap);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; t++) f[t] = 1.f;
+        }
+        if (j0 < w_lo_max || j0 + KV_PAGE > w_hi_min) {
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+                const int j = j0 + 8 * (i / 4) + 4 * h + i % 4;
+                if (j < lo || j >= hi) s[i / 16][i % 16] = MINUS_INF;
+            }
+        }
+        float top = MINUS_INF;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {  // 16 tokens of one scale
+            float x = s[t / 2][8 * (t % 2)];
+#pragma unroll
+            for (int i = 1; i < 8; i++) x = fmaxf(x, s[t / 2][8 * (t % 2) + i]);
+            top = fmaxf(top, x * f[t]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float m_new = fmaxf(m, top), base = m_new == MINUS_INF ? 0.f : m_new;
+        float keep = __builtin_amdgcn_exp2f(m - base);
+        l *= keep;
+        if (vmax > ref) {
+            const float up = pow2(min(exponent(vmax) + 1, 126));
+            keep *= ref / up;
+            ref = up;
+        }
+        m = m_new;
+        if (__ballot(keep != 1.f)) {
+#pragma unroll
+            for (int d = 0; d < 2 * NC; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) acc[d][i] *= keep;
+        }
+        Halves ph[4], pl[PHILO ? 4 : 1];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const float wt = w[t] * (0x1p15f / ref);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float z = s[t / 2][8 * (t % 2) + i];
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z, f[t], -base));
+                l += p;
+                float y = p * wt;
+                if (PHILO) y = settled(y);
+                const _Float16 x = (_Float16)y;
+                ph[t].v[i] = x;
+                if (PHILO) pl[PHILO ? t : 0].v[i] = (_Float16)(y - (float)x);
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < 2 * NC; d++) {
+            const uint4 x0 = *(const uint4 *)(vb + ((2 * d + r / 16) * 64 + h * 16 + r % 16) * 16);
+            const uint4 x1 = *(const uint4 *)(vb + ((2 * d + r / 16) * 64 + (h + 2) * 16 + r % 16) * 16);
+            const uint32_t a0[4] = {x0.x, x0.y, x0.z, x0.w}, a1[4] = {x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const half8 v = widen_centred(a0[t], a1[t]);
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[t].v, acc[d], 0, 0, 0);
+                if (PHILO) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[PHILO ? t : 0].v, acc[d], 0, 0, 0);
+            }
+        }
+    }
+
+    l += __shfl_xor(l, 32);
+    if (!valid) return;
+    const int o_h = head * a.group + my_h;
+    const float base = m == MINUS_INF ? 0.f : m;
+    float weight = ref * 0x1p-15f;
+    float *part = a.part + (((int64_t)item * a.c.kv_heads + head) * a.splits + blockIdx.z) * (TILE * (DP + 2));
+    const int in_tile = 32 * wave + r;
+    if (a.splits == 1) {
+        float total = l, scale = 1.f;
+        if (a.sinks) {
+            const float sink = a.sinks[o_h] * LOG2E, all = fmaxf(base, sink);
+            scale = __builtin_amdgcn_exp2f(base - all);
+            total = l * scale + __builtin_amdgcn_exp2f(sink - all);
+        }
+        weight = l == 0.f ? 0.f : weight * (scale / total);
+    } else if (h == 0) {
+        part[TILE * DP + in_tile] = m;
+        part[TILE * DP + TILE + in_tile] = l;
+    }
+    T *out = (T *)a.out + (int64_t)(begin + my_t) * a.out_stride + (int64_t)o_h * a.c.head_dim;
+#pragma unroll
+    for (int d = 0; d < 2 * NC; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int at = 32 * d + 8 * i + 4 * h;
+            if (at >= a.c.head_dim) continue;
+            float4v y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = l == 0.f ? 0.f : acc[d][4 * i + e] * weight;
+            if (a.splits == 1) {
+                V4 z;
+#pragma unroll
+                for (int e = 0; e < 4; e++) z[e] = (T)y[e];
+                *(V4 *)(out + at) = z;
+            } else {
+                *(float4v *)(part + in_tile * DP + at) = y;
+            }
+        }
+}
+
 // the splits of a tile joined: a thread takes four dimensions of one row
-template <class T>
+template <class T, int R>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnLaunch a) {
     using V4 = typename Vec4<T>::type;
     const int head = blockIdx.y, dp = a.c.dp, quads = a.c.head_dim / 4;
     int seq, tile, begin;
-    auto tiles = [&](int s) { int x; const int n = seq_rows(a.b, s, x); return (int)(((int64_t)n * a.group + ROWS - 1) / ROWS); };
-    if (!find_item(a.b.n_seqs, (int)blockIdx.x, tiles, seq, tile)) return;
+    if (!find_item(a.b.n_seqs, (int)blockIdx.x, [&](int s) { return tiles_of<R>(a, s); }, seq, tile)) return;
     const int n = seq_rows(a.b, seq, begin);
-    const int rows = min(ROWS, n * a.group - tile * ROWS);
-    const int64_t size = ROWS * (dp + 2);
+    const int rows = min(R, n * a.group - tile * R);
+    const int64_t size = R * (dp + 2);
     const float *part = a.part + ((int64_t)blockIdx.x * a.c.kv_heads + head) * a.splits * size;
     for (int i = threadIdx.x; i < rows * quads; i += 256) {
         const int row = i / quads, d = (i - row * quads) * 4;
-        const int t = (tile * ROWS + row) / a.group, h = head * a.group + tile * ROWS + row - t * a.group;
+        const int t = (tile * R + row) / a.group, h = head * a.group + tile * R + row - t * a.group;
         float top = MINUS_INF;
-        for (int s = 0; s < a.splits; s++) top = fmaxf(top, part[s * size + ROWS * dp + row]);
+        for (int s = 0; s < a.splits; s++) top = fmaxf(top, part[s * size + R * dp + row]);
         const float sink = a.sinks ? a.sinks[h] * LOG2E : MINUS_INF;
         top = fmaxf(top, sink);
         const float base = top == MINUS_INF ? 0.f : top;
         float sum = 0.f;
         float4v y = {0.f, 0.f, 0.f, 0.f};
         for (int s = 0; s < a.splits; s++) {
-            const float l = part[s * size + ROWS * dp + ROWS + row];
+            const float l = part[s * size + R * dp + R + row];
             if (l == 0.f) continue;  // a split that saw nothing
-            const float w = __builtin_amdgcn_exp2f(part[s * size + ROWS * dp + row] - base);
+            const float w = __builtin_amdgcn_exp2f(part[s * size + R * dp + row] - base);
             const float4v x = *(const float4v *)(part + s * size + row * dp + d);
             sum += l * w;
 #pragma unroll
@@ -378,64 +664,124 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnLaunch a) {
     }
 }
 
-template <class T, int NC>
-hipError_t launch_rows(const AttnLaunch &a, dim3 grid, hipStream_t s) {
-    if (a.softcap > 0.f) attn_rows_kernel<T, NC, true><<<grid, 256, 0, s>>>(a);
-    else attn_rows_kernel<T, NC, false><<<grid, 256, 0, s>>>(a);
-    return hipGetLastError();
-}
-
-template <class T>
-hipError_t launch_t(const AttnLaunch &a, dim3 grid, hipStream_t s) {
-    hipError_t e;
-    switch (a.c.dp / 64) {
-    case 1: e = launch_rows<T, 1>(a, grid, s); break;
-    case 2: e = launch_rows<T, 2>(a, grid, s); break;
-    case 3: e = launch_rows<T, 3>(a, grid, s); break;
-    default: e = launch_rows<T, 4>(a, grid, s); break;
+template <class T, int NC, int R>
+hipError_t launch_one(const AttnLaunch &a, hipStream_t s) {
+    if (R == ROWS) {
+        const dim3 grid((unsigned)a.items, (unsigned)a.c.kv_heads, (unsigned)a.splits);
+        if (a.softcap > 0.f) attn_rows_kernel<T, NC, true><<<grid, 256, 0, s>>>(a);
+        else attn_rows_kernel<T, NC, false><<<grid, 256, 0, s>>>(a);
+    } else {
+        const dim3 grid((unsigned)a.items * (unsigned)a.c.kv_heads, 1, (unsigned)a.splits);
+        if (a.softcap > 0.f) attn_tile_kernel<T, NC, true><<<grid, 256, 0, s>>>(a);
+        else attn_tile_kernel<T, NC, false><<<grid, 256, 0, s>>>(a);
     }
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
-    attn_join_kernel<T><<<dim3(grid.x, grid.y), 256, 0, s>>>(a);
+    attn_join_kernel<T, R><<<dim3((unsigned)a.items, (unsigned)a.c.kv_heads), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 
-struct Plan { int64_t items; int splits; };
-
-// Row tiles at most, and workgroups per tile: the cache of a tile is cut until about eight workgroups per CU run (rounds
-// of them even out sequences of different lengths), down to one page per wave.
-Plan plan_of(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus) {
-    const int64_t group = d.n_heads / c.kv_heads;
-    const int64_t active = b.n_seqs < b.n_rows ? b.n_seqs : b.n_rows;
-    Plan p;
-    p.items = (b.n_rows * group + (ROWS - 1) * active) / ROWS;
-    int64_t pages = b.max_pages;
-    if (d.window > 0) {  // a tile's rows are ROWS / group tokens at most one after the other
-        const int64_t w = ((int64_t)d.window + ROWS) / KV_PAGE + 2;
-        if (d.causal && w < pages) pages = w;
+template <class T, int R>
+hipError_t launch_t(const AttnLaunch &a, hipStream_t s) {
+    switch (a.c.dp / 64) {
+    case 1: return launch_one<T, 1, R>(a, s);
+    case 2: return launch_one<T, 2, R>(a, s);
+    case 3: return launch_one<T, 3, R>(a, s);
+    default: return launch_one<T, 4, R>(a, s);
     }
-    const int64_t want = 8ll * num_cus / (p.items * c.kv_heads) + 1, most = (pages + 3) / 4;
-    p.splits = (int)(want < most ? want : most);
-    if (p.splits < 1) p.splits = 1;
-    if (p.splits > 256) p.splits = 256;
-    return p;
+}
+
+template <int R>
+hipError_t launch_type(const AttnLaunch &a, int type, hipStream_t s) {
+    if (type == T_F32) return launch_t<float, R>(a, s);
+    if (type == T_F16) return launch_t<_Float16, R>(a, s);
+    return launch_t<__bf16, R>(a, s);
+}
+
+// Sequences of at most FEW (token, head) rows per key/value head go to the 16-row kernel, longer ones to the 128-row one.
+constexpr int FEW = 32;
+
+struct Plan {
+    int64_t items;  // tiles at most; 0: no launch
+    int splits, least, most;
+    size_t floats;  // of partial results
+};
+
+// Splits of the cache that a tile's workgroups share, for `work` workgroups without and `slots` that run at a time.
+// pages: what a tile may see.  Cost of s splits: rounds of workgroups times their share, and a little for the join.
+int splits_for(int64_t work, int64_t slots, int64_t pages, int most) {
+    int best = 1;
+    double least = 0;
+    for (int s = 1; s <= most && (s == 1 || s * 4 <= pages); s++) {
+        const int64_t rounds = (work * s + slots - 1) / slots;
+        const double cost = (double)rounds / s * (1 + 0.03 * (s - 1)) ;
+        if (s == 1 || cost < least) { best = s; least = cost; }
+    }
+    return best;
+}
+
+void plans_of(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus, Plan &few, Plan &many) {
+    const int64_t group = d.n_heads / c.kv_heads, all = b.n_rows * group;
+    const int64_t active = b.n_seqs < b.n_rows ? b.n_seqs : b.n_rows;
+    few = many = Plan{0, 1, 1, INT32_MAX, 0};
+    // a row per sequence or few in all: the 16-row kernel; one sequence: either; otherwise both kernels look for theirs
+    const bool some_many = all > FEW && b.n_rows > b.n_seqs, some_few = b.n_seqs > 1 || !some_many;
+    if (some_few) {
+        few.items = (all + (ROWS - 1) * active) / ROWS;
+        if (some_many) {
+            few.most = FEW;
+            const int64_t cap = active * ((FEW + ROWS - 1) / ROWS);
+            if (few.items > cap) few.items = cap;
+        }
+        int64_t pages = b.max_pages;
+        if (d.window > 0 && d.causal) {  // a tile's rows are at most 16 tokens one after the other
+            const int64_t w = ((int64_t)d.window + ROWS) / KV_PAGE + 2;
+            if (w < pages) pages = w;
+        }
+        // about eight workgroups per CU (rounds of them even out sequences of different lengths), down to a page per wave
+        const int64_t want = 8ll * num_cus / (few.items * c.kv_heads) + 1, most = (pages + 3) / 4;
+        few.splits = (int)(want < most ? want : most);
+        if (few.splits < 1) few.splits = 1;
+        if (few.splits > 256) few.splits = 256;
+        if (few.splits > 1) few.floats = (size_t)few.items * c.kv_heads * few.splits * (ROWS * (size_t)(c.dp + 2));
+    }
+    if (some_many) {
+        const int64_t seqs = all / (FEW + 1) < active ? all / (FEW + 1) : active;  // sequences that can be longer than FEW
+        many.items = (all + (TILE - 1) * seqs) / TILE;
+        if (b.n_seqs > 1) many.least = FEW + 1;
+        int64_t pages = b.max_pages;
+        if (d.window > 0 && d.causal) {
+            const int64_t w = ((int64_t)d.window + TILE) / KV_PAGE + 2;
+            if (w < pages) pages = w;
+        }
+        many.splits = splits_for(many.items * c.kv_heads, (c.dp <= 128 ? 2 : 1) * num_cus, pages, 16);
+        if (many.splits > 1) many.floats = (size_t)many.items * c.kv_heads * many.splits * (TILE * (size_t)(c.dp + 2));
+    }
 }
 
 }  // namespace
 
 size_t attn_workspace_floats(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus) {
-    const Plan p = plan_of(c, b, d, num_cus);
-    return p.splits == 1 ? 0 : (size_t)p.items * c.kv_heads * p.splits * (ROWS * (size_t)(c.dp + 2));
+    Plan few, many;
+    plans_of(c, b, d, num_cus, few, many);
+    return few.floats + many.floats;
 }
 
 hipError_t launch_attention(const DevKv &c, const DevBatch &b, const AttnDesc &d, const void *q, int64_t q_stride, void *out,
                             int64_t out_stride, float *workspace, int num_cus, hipStream_t s) {
-    const Plan p = plan_of(c, b, d, num_cus);
+    Plan few, many;
+    plans_of(c, b, d, num_cus, few, many);
     AttnLaunch a{c, b, q, out, q_stride, out_stride, d.n_heads, d.n_heads / c.kv_heads, d.scale, d.softcap, d.causal, d.window,
-                 d.sinks, workspace, p.splits};
-    const dim3 grid((unsigned)p.items, (unsigned)c.kv_heads, (unsigned)p.splits);
-    if (d.type == T_F32) return launch_t<float>(a, grid, s);
-    if (d.type == T_F16) return launch_t<_Float16>(a, grid, s);
-    return launch_t<__bf16>(a, grid, s);
+                 d.sinks, nullptr, 1, 0, 0, 0};
+    for (int i = 0; i < 2; i++) {
+        const Plan &p = i ? few : many;
+        if (!p.items) continue;
+        a.part = workspace + (i ? many.floats : 0);
+        a.splits = p.splits; a.items = (int)p.items; a.most = p.most; a.least = p.least;
+        const hipError_t e = i ? launch_type<ROWS>(a, d.type, s) : launch_type<TILE>(a, d.type, s);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace miqmm

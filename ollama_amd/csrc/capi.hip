@@ -1990,7 +1990,7 @@ int value_size(int type) { return type == T_F32 ? 4 : type == T_F16 || type == T
 int check_values(int type, int64_t n, int location) {
     if (!value_size(type)) return fail(MI_QMM_ERR_UNSUPPORTED, "type %d is not F32 (0), F16 (1) or BF16 (30)", type);
     if (n < 0) return fail(MI_QMM_ERR_INVALID, "n=%lld must be non-negative", (long long)n);
-    if (n > (1 << 24)) return fail(MI_QMM_ERR_UNSUPPORTED, "n=%lld: at most 2^24 rows", (long long)n);
+    if (n > (1 << 22)) return fail(MI_QMM_ERR_UNSUPPORTED, "n=%lld: at most 2^22 rows", (long long)n);
     if (location != MI_QMM_HOST && location != MI_QMM_DEVICE)
         return fail(MI_QMM_ERR_INVALID, "location must be MI_QMM_HOST or MI_QMM_DEVICE");
     return MI_QMM_OK;
@@ -2289,7 +2289,7 @@ int mi_qmm_attention(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *b
     if (p->n_heads < 1 || p->n_heads > 65535 || p->n_heads % c.kv_heads)
         return fail(MI_QMM_ERR_INVALID, "n_heads=%d is no multiple of the cache's %d heads", p->n_heads, c.kv_heads);
     if (!(p->softcap >= 0.f) || p->window < 0) return fail(MI_QMM_ERR_INVALID, "softcap=%g window=%d must be non-negative", (double)p->softcap, p->window);
-    if (n * (p->n_heads / c.kv_heads) > (1 << 27)) return fail(MI_QMM_ERR_UNSUPPORTED, "n=%lld rows of %d heads", (long long)n, p->n_heads);
+    if (n * p->n_heads > (1 << 27)) return fail(MI_QMM_ERR_UNSUPPORTED, "n=%lld rows of %d heads", (long long)n, p->n_heads);
     if (n == 0 || b->n_seqs == 0) return MI_QMM_OK;
     if ((rc = check_rows("q", q, q_stride, p->n_heads, c.head_dim, p->type, location)) ||
         (rc = check_rows("out", out, out_stride, p->n_heads, c.head_dim, p->type, location)))
