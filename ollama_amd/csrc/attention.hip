@@ -48,6 +48,7 @@ struct AttnLaunch {
     const float *sinks;
     float *part;  // [item][kv head][split]: R x dp numerators, R maxima, R sums (R rows per tile)
     int splits, items;
+    int shift;        // groups of 16 tokens per scale, as a power of two
     int most, least;  // sequences of least..most (token, head) rows per key/value head are this launch's
 };
 
@@ -104,6 +105,26 @@ __device__ __forceinline__ void visible(const AttnLaunch &a, int pos, int len, i
     hi = max(hi, 0);
 }
 
+// a / b where both are the same for the whole wave (a division is vector code: its result goes back to a scalar register)
+__device__ __forceinline__ int same(int a, int b) { return __builtin_amdgcn_readfirstlane(a / b); }
+
+// the page that holds tokens 64 page .. 64 page + 63 of sequence seq; -1: there is none
+__device__ __forceinline__ int page_of(const AttnLaunch &a, int seq, int page) {
+    const int phys = page < a.b.max_pages ? fixed(a.b.pages + (int64_t)seq * a.b.max_pages + page) : -1;
+    return phys < a.c.n_pages ? phys : -1;
+}
+
+// the scales of its groups of 16 tokens; NaN where there is no such page: whoever sees it gets NaN
+__device__ __forceinline__ void scales_of(const AttnLaunch &a, int64_t at, bool bad, float (&ks)[4], float (&vs)[4]) {
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+        const int64_t i = at * a.c.per + (t >> a.shift);
+        const float k = fixed(a.c.ks + i), v = fixed(a.c.vs + i);
+        ks[t] = bad ? __builtin_nanf("") : k;
+        vs[t] = bad ? __builtin_nanf("") : v;
+    }
+}
+
 // Scales that are no numbers (a poisoned block, a page that there is not) are taken out of a page's work -- masked tokens of
 // such a block would turn into NaN -- and make NaN of the sum of a row (lo .. hi - 1) that sees one of the block's tokens.
 __device__ __forceinline__ void take_out_nan(float (&ks)[4], float (&vs)[4], int j0, int lo, int hi, float &l) {
@@ -138,15 +159,15 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
     int seq, tile;
     if (!find_item(a.b.n_seqs, (int)blockIdx.x, [&](int s) { return tiles_of<ROWS>(a, s); }, seq, tile)) return;
     int begin;
-    const int n = seq_rows(a.b, seq, begin), len = a.b.kv_len[seq], first = len - n;
+    const int n = seq_rows(a.b, seq, begin), len = fixed(a.b.kv_len + seq), first = len - n;
     const int rows = n * a.group, row0 = tile * ROWS;
     const bool valid = row0 + r < rows;
     const int my_t = valid ? (row0 + r) / a.group : 0, my_h = valid ? row0 + r - my_t * a.group : 0;
     int lo, hi;
     visible(a, first + my_t, len, lo, hi);
     int lo_min, lo_max, hi_min, hi_max;  // over the tile's rows: both bounds grow with the row
-    visible(a, first + row0 / a.group, len, lo_min, hi_min);
-    visible(a, first + (min(row0 + ROWS, rows) - 1) / a.group, len, lo_max, hi_max);
+    visible(a, first + same(row0, a.group), len, lo_min, hi_min);
+    visible(a, first + same(min(row0 + ROWS, rows) - 1, a.group), len, lo_max, hi_max);
 
     // queries: dimensions 64 c + 16 g + 8 i .. + 7 of row r, as the second operand of step (c, i)
     Halves qh[2 * NC], ql[2 * NC];
@@ -195,19 +216,17 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
 #pragma unroll
     for (int i = 0; i < 4 * NC; i++) acc[i] = float4v{0.f, 0.f, 0.f, 0.f};
     float m = MINUS_INF, l = 0.f;
-    float ref = 0x1p-100f;  // values are accumulated in units of ref * 2^-15
+    float ref = 0x1p-100f, unit = 0x1p115f;  // values are accumulated in units of ref * 2^-15 = 1 / unit
 
     int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
     if (a.splits > 1) {
-        const int share = (t1 - t0 + a.splits - 1) / a.splits;
+        const int share = same(t1 - t0 + a.splits - 1, a.splits);
         t0 = t0 + (int)blockIdx.z * share;
         t1 = min(t1, t0 + share);
     }
     for (int page = t0 + wave; page < t1; page += 4) {
-        int64_t phys = page < a.b.max_pages ? a.b.pages[(int64_t)seq * a.b.max_pages + page] : -1;
-        const bool bad = phys < 0 || phys >= a.c.n_pages;  // no such page: whoever sees it gets NaN
-        if (bad) phys = 0;
-        const int64_t at = phys * a.c.kv_heads + head;
+        const int phys = page_of(a, seq, page);
+        const int64_t at = (int64_t)max(phys, 0) * a.c.kv_heads + head;
         const uint4 *kp = (const uint4 *)(a.c.k + at * (KV_PAGE * DP)) + lane;
         const uint4 *vp = (const uint4 *)(a.c.v + at * (KV_PAGE * DP)) + lane;
         uint4 kc[4][NC], vc[4 * NC];
@@ -218,12 +237,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
 #pragma unroll
         for (int d = 0; d < 4 * NC; d++) vc[d] = vp[d * 64];
         float ks[4], vs[4];
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const int64_t i = at * a.c.per + 16 * t / a.c.block;
-            ks[t] = bad ? __builtin_nanf("") : a.c.ks[i];
-            vs[t] = bad ? __builtin_nanf("") : a.c.vs[i];
-        }
+        scales_of(a, at, phys < 0, ks, vs);
         const int j0 = page * KV_PAGE;
         take_out_nan(ks, vs, j0, lo, hi, l);
         float z[16];
@@ -265,9 +279,10 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
         float keep = __builtin_amdgcn_exp2f(m - base);
         l *= keep;
         if (vmax > ref) {
-            const float up = pow2(min(exponent(vmax) + 1, 126));
-            keep *= ref / up;
-            ref = up;
+            const int e = min(exponent(vmax) + 1, 126);
+            keep *= ref * pow2(-e);
+            ref = pow2(e);
+            unit = e >= -100 ? pow2(15 - e) : unit;
         }
         m = m_new;
         if (__ballot(keep != 1.f)) {
@@ -281,7 +296,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
         for (int i = 0; i < 16; i++) {
             const float p = __builtin_amdgcn_exp2f(z[i] - base);
             l += p;
-            float y = p * (vs[i / 4] * (0x1p15f / ref));
+            float y = p * (vs[i / 4] * unit);
             if (PHILO) y = settled(y);
             const _Float16 h = (_Float16)y;
             ph[i / 8].v[i % 8] = h;
@@ -388,16 +403,16 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
     int seq, tile;
     if (!find_item(a.b.n_seqs, item, [&](int s) { return tiles_of<TILE>(a, s); }, seq, tile)) return;
     int begin;
-    const int n = seq_rows(a.b, seq, begin), len = a.b.kv_len[seq], first = len - n;
+    const int n = seq_rows(a.b, seq, begin), len = fixed(a.b.kv_len + seq), first = len - n;
     const int rows = n * a.group, row0 = tile * TILE, wrow0 = row0 + 32 * wave;
     const bool valid = wrow0 + r < rows;
     const int my_t = valid ? (wrow0 + r) / a.group : 0, my_h = valid ? wrow0 + r - my_t * a.group : 0;
     int lo, hi, lo_min, lo_max, hi_min, hi_max, w_lo_min, w_lo_max, w_hi_min, w_hi_max;
     visible(a, first + my_t, len, lo, hi);
-    visible(a, first + row0 / a.group, len, lo_min, hi_min);
-    visible(a, first + (min(row0 + TILE, rows) - 1) / a.group, len, lo_max, hi_max);
-    visible(a, first + min(wrow0, rows - 1) / a.group, len, w_lo_min, w_hi_min);
-    visible(a, first + (min(wrow0 + 32, rows) - 1) / a.group, len, w_lo_max, w_hi_max);
+    visible(a, first + same(row0, a.group), len, lo_min, hi_min);
+    visible(a, first + same(min(row0 + TILE, rows) - 1, a.group), len, lo_max, hi_max);
+    visible(a, first + same(min(wrow0, rows - 1), a.group), len, w_lo_min, w_hi_min);
+    visible(a, first + same(min(wrow0 + 32, rows) - 1, a.group), len, w_lo_max, w_hi_max);
 
     // queries: dimensions 64 c + 16 (2 e + h) + 8 i .. + 7 of row r, as the second operand of step (c, e, i)
     Halves qh[NC][2][2], ql[HILO ? NC : 1][2][2];
@@ -443,56 +458,47 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
     for (int d = 0; d < 2 * NC; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
-    float m = MINUS_INF, l = 0.f, ref = 0x1p-100f;
+    float m = MINUS_INF, l = 0.f;
+    float ref = 0x1p-100f, unit = 0x1p115f;  // values are accumulated in units of ref * 2^-15 = 1 / unit
 
     int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
     if (a.splits > 1) {
-        const int share = (t1 - t0 + a.splits - 1) / a.splits;
+        const int share = same(t1 - t0 + a.splits - 1, a.splits);
         t0 = t0 + (int)blockIdx.z * share;
         t1 = min(t1, t0 + share);
     }
-    // a page's number, two pages ahead of its use: the number, then its codes and scales, then the work
-    auto page_at = [&](int page) {
-        const int64_t phys = page < t1 && page < a.b.max_pages ? a.b.pages[(int64_t)seq * a.b.max_pages + page] : -1;
-        return phys < a.c.n_pages ? phys : -1;
-    };
     float ks[4], vs[4];
-    auto fetch = [&](int64_t phys, int b) {
-        const bool bad = phys < 0;  // no such page: whoever sees it gets NaN
-        const int64_t at = (bad ? 0 : phys) * a.c.kv_heads + head;
+    auto fetch = [&](int phys, int b) {
+        const int64_t at = (int64_t)max(phys, 0) * a.c.kv_heads + head;
 #pragma unroll
         for (int i = 0; i < NC; i++) {
             const int kb = (wave * NC + i) * 1024;
             __builtin_amdgcn_global_load_lds((glb_ptr_t *)(a.c.k + at * BYTES + kb + lane * 16), (lds_ptr_t *)(buf[b] + kb), 16, 0, 0);
             __builtin_amdgcn_global_load_lds((glb_ptr_t *)(a.c.v + at * BYTES + kb + lane * 16), (lds_ptr_t *)(buf[b] + BYTES + kb), 16, 0, 0);
         }
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const int64_t i = at * a.c.per + 16 * t / a.c.block;
-            ks[t] = bad ? __builtin_nanf("") : a.c.ks[i];
-            vs[t] = bad ? __builtin_nanf("") : a.c.vs[i];
-        }
+        scales_of(a, at, phys < 0, ks, vs);
     };
-    int64_t next = page_at(t0);
-    if (t0 < t1) fetch(next, 0);
-    next = page_at(t0 + 1);
+    // a page's number two pages ahead of its use: the number, then its codes and scales, then the work
+    if (t0 < t1) fetch(page_of(a, seq, t0), 0);
+    int next = page_of(a, seq, t0 + 1);
     for (int page = t0; page < t1; page++) {
         const int b = (page - t0) & 1;
         const int j0 = page * KV_PAGE;
         take_out_nan(ks, vs, j0, lo, hi, l);
-        float f[4], w[4];
+        float f[4], w[4], off[4];  // a score is s * f + off
         const float vmax = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             f[t] = score_scale * ks[t];
             if (f[t] == 0.f) f[t] = 1e-30f;  // times a masked token's -inf stays -inf; all else is 0 either way
+            off[t] = HILO ? 0.f : minus_bias * f[t];
             w[t] = vs[t];
         }
         __builtin_amdgcn_s_waitcnt((0 & 15) | (7 << 4) | (15 << 8));  // vmcnt(0): this wave's part of the page is in LDS
         __syncthreads();
         if (page + 1 < t1) {
             fetch(next, b ^ 1);
-            next = page_at(page + 2);
+            next = page_of(a, seq, page + 2);
         }
         if (wrow0 >= rows || j0 >= w_hi_max || j0 + KV_PAGE <= w_lo_min) continue;  // nothing that this wave's rows see
         const uint8_t *kb = buf[b], *vb = buf[b] + BYTES;
@@ -500,7 +506,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
 #pragma unroll
         for (int t = 0; t < 2; t++) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[t][i] = minus_bias;
+            for (int i = 0; i < 16; i++) s[t][i] = 0.f;
 #pragma unroll
             for (int c = 0; c < NC; c++)
 #pragma unroll
@@ -520,10 +526,10 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
 #pragma unroll
             for (int i = 0; i < 32; i++) {
                 const int t = i / 8;
-                s[i / 16][i % 16] = a.softcap * LOG2E * tanhf(s[i / 16][i % 16] * f[t] / a.softcap);
+                s[i / 16][i % 16] = a.softcap * LOG2E * tanhf(__builtin_fmaf(s[i / 16][i % 16], f[t], off[t]) / a.softcap);
             }
 #pragma unroll
-            for (int t = 0; t < 4; t++) f[t] = 1.f;
+            for (int t = 0; t < 4; t++) { f[t] = 1.f; off[t] = 0.f; }
         }
         if (j0 < w_lo_max || j0 + KV_PAGE > w_hi_min) {
 #pragma unroll
@@ -538,16 +544,17 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
             float x = s[t / 2][8 * (t % 2)];
 #pragma unroll
             for (int i = 1; i < 8; i++) x = fmaxf(x, s[t / 2][8 * (t % 2) + i]);
-            top = fmaxf(top, x * f[t]);
+            top = fmaxf(top, __builtin_fmaf(x, f[t], off[t]));
         }
         top = fmaxf(top, __shfl_xor(top, 32));
         const float m_new = fmaxf(m, top), base = m_new == MINUS_INF ? 0.f : m_new;
         float keep = __builtin_amdgcn_exp2f(m - base);
         l *= keep;
         if (vmax > ref) {
-            const float up = pow2(min(exponent(vmax) + 1, 126));
-            keep *= ref / up;
-            ref = up;
+            const int e = min(exponent(vmax) + 1, 126);
+            keep *= ref * pow2(-e);
+            ref = pow2(e);
+            unit = e >= -100 ? pow2(15 - e) : unit;
         }
         m = m_new;
         if (__ballot(keep != 1.f)) {
@@ -559,11 +566,11 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
         Halves ph[4], pl[PHILO ? 4 : 1];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            const float wt = w[t] * (0x1p15f / ref);
+            const float wt = w[t] * unit, shift = off[t] - base;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const float z = s[t / 2][8 * (t % 2) + i];
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z, f[t], -base));
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z, f[t], shift));
                 l += p;
                 float y = p * wt;
                 if (PHILO) y = settled(y);
@@ -707,17 +714,13 @@ struct Plan {
     size_t floats;  // of partial results
 };
 
-// Splits of the cache that a tile's workgroups share, for `work` workgroups without and `slots` that run at a time.
-// pages: what a tile may see.  Cost of s splits: rounds of workgroups times their share, and a little for the join.
-int splits_for(int64_t work, int64_t slots, int64_t pages, int most) {
-    int best = 1;
-    double least = 0;
-    for (int s = 1; s <= most && (s == 1 || s * 4 <= pages); s++) {
-        const int64_t rounds = (work * s + slots - 1) / slots;
-        const double cost = (double)rounds / s * (1 + 0.03 * (s - 1)) ;
-        if (s == 1 || cost < least) { best = s; least = cost; }
-    }
-    return best;
+// Splits of the cache for `work` workgroups without, `slots` of which run at a time.  Tiles that fill the device are not
+// split (a split tile's partial results are written and read once more, at 128 rows a third of the kernel's own time on
+// prompts of 4096); fewer are, so that they fill it, while a split keeps four pages.
+int splits_for(int64_t work, int64_t slots, int64_t pages) {
+    int64_t s = slots / work;
+    if (s > pages / 4) s = pages / 4;
+    return s < 1 ? 1 : s > 32 ? 32 : (int)s;
 }
 
 void plans_of(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus, Plan &few, Plan &many) {
@@ -754,7 +757,7 @@ void plans_of(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus,
             const int64_t w = ((int64_t)d.window + TILE) / KV_PAGE + 2;
             if (w < pages) pages = w;
         }
-        many.splits = splits_for(many.items * c.kv_heads, (c.dp <= 128 ? 2 : 1) * num_cus, pages, 16);
+        many.splits = splits_for(many.items * c.kv_heads, (c.dp <= 128 ? 2 : 1) * num_cus, pages);
         if (many.splits > 1) many.floats = (size_t)many.items * c.kv_heads * many.splits * (TILE * (size_t)(c.dp + 2));
     }
 }
@@ -772,7 +775,7 @@ hipError_t launch_attention(const DevKv &c, const DevBatch &b, const AttnDesc &d
     Plan few, many;
     plans_of(c, b, d, num_cus, few, many);
     AttnLaunch a{c, b, q, out, q_stride, out_stride, d.n_heads, d.n_heads / c.kv_heads, d.scale, d.softcap, d.causal, d.window,
-                 d.sinks, nullptr, 1, 0, 0, 0};
+                 d.sinks, nullptr, 1, 0, c.block == 16 ? 0 : c.block == 32 ? 1 : 2, 0, 0};
     for (int i = 0; i < 2; i++) {
         const Plan &p = i ? few : many;
         if (!p.items) continue;

@@ -34,10 +34,16 @@ struct DevBatch {
     int n_rows;
 };
 
+// *p as a scalar load where p is the same for the whole wave: nothing that a kernel reads this way is written by it
+template <class T>
+__device__ __forceinline__ T fixed(const T *p) {
+    return *(const __attribute__((address_space(4))) T *)p;
+}
+
 // rows of sequence s and the first of them; a range that is no part of 0..n_rows counts as none
 __device__ __forceinline__ int seq_rows(const DevBatch &b, int s, int &begin) {
-    begin = b.row_start[s];
-    const int end = b.row_start[s + 1];
+    begin = fixed(b.row_start + s);
+    const int end = fixed(b.row_start + s + 1);
     return begin >= 0 && end <= b.n_rows && end > begin ? end - begin : 0;
 }
 
@@ -60,8 +66,8 @@ __device__ __forceinline__ bool find_item(int n_seqs, int item, F count, int &se
         if (item < base + total) {
             const unsigned long long past = __ballot(base + incl > item);
             const int at = __builtin_ctzll(past);
-            seq = s0 + at;
-            local = item - base - __builtin_amdgcn_readlane(incl - c, at);
+            seq = __builtin_amdgcn_readfirstlane(s0 + at);
+            local = __builtin_amdgcn_readfirstlane(item - base - __builtin_amdgcn_readlane(incl - c, at));
             return true;
         }
         base += total;
