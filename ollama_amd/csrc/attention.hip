@@ -105,6 +105,30 @@ __device__ __forceinline__ void visible(const AttnLaunch &a, int pos, int len, i
     hi = max(hi, 0);
 }
 
+// cap(z) in units of log2 for N scores x / softcap: c log2(e) tanh(x).  Below 0.35 the odd series to x^11 (2e-8 of the value;
+// the formula with the exponential would lose eight bits there), and where no lane of the wave has more, that alone.
+template <int N>
+__device__ __forceinline__ void cap_scores(float (&x)[N], float c) {
+    float big = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; i++) big = fmaxf(big, fabsf(x[i]));
+    if (__ballot(!(big < 0.35f)) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float y = x[i] * x[i];
+            float p = __builtin_fmaf(y, -1382.f / 155925.f, 62.f / 2835.f);
+            p = __builtin_fmaf(y, p, -17.f / 315.f);
+            p = __builtin_fmaf(y, p, 2.f / 15.f);
+            p = __builtin_fmaf(y, p, -1.f / 3.f);
+            const float cx = c * x[i];
+            x[i] = __builtin_fmaf(cx * y, p, cx);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = c * tanhf(x[i]);
+    }
+}
+
 // a / b where both are the same for the whole wave (a division is vector code: its result goes back to a scalar register)
 __device__ __forceinline__ int same(int a, int b) { return __builtin_amdgcn_readfirstlane(a / b); }
 
@@ -209,7 +233,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
         minus_bias = HILO ? 0.f : sum * (-128.f * 0x1p-24f);
-        score_scale = a.scale * (HILO ? 1.f : 0x1p24f) * pow2(-e) * (CAP ? 1.f : LOG2E);
+        score_scale = a.scale * (HILO ? 1.f : 0x1p24f) * pow2(-e) * (CAP ? 1.f / a.softcap : LOG2E);
     }
 
     float4v acc[4 * NC];
@@ -257,11 +281,9 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
             }
             const float f = score_scale * ks[t];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                z[4 * t + i] = s[i] * f;
-                if (CAP) z[4 * t + i] = a.softcap * LOG2E * tanhf(z[4 * t + i] / a.softcap);
-            }
+            for (int i = 0; i < 4; i++) z[4 * t + i] = s[i] * f;
         }
+        if (CAP) cap_scores(z, a.softcap * LOG2E);
         if (j0 < lo_max || j0 + KV_PAGE > hi_min) {
 #pragma unroll
             for (int i = 0; i < 16; i++) {
@@ -450,7 +472,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
             }
         sum += __shfl_xor(sum, 32);
         minus_bias = HILO ? 0.f : sum * (-128.f * 0x1p-24f);
-        score_scale = fabsf(a.scale) * (HILO ? 1.f : 0x1p24f) * pow2(-e) * (CAP ? 1.f : LOG2E);
+        score_scale = fabsf(a.scale) * (HILO ? 1.f : 0x1p24f) * pow2(-e) * (CAP ? 1.f / a.softcap : LOG2E);
     }
 
     float16v acc[2 * NC];
@@ -523,11 +545,12 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
                 }
         }
         if (CAP) {
+            float x[32];
 #pragma unroll
-            for (int i = 0; i < 32; i++) {
-                const int t = i / 8;
-                s[i / 16][i % 16] = a.softcap * LOG2E * tanhf(__builtin_fmaf(s[i / 16][i % 16], f[t], off[t]) / a.softcap);
-            }
+            for (int i = 0; i < 32; i++) x[i] = __builtin_fmaf(s[i / 16][i % 16], f[i / 8], off[i / 8]);
+            cap_scores(x, a.softcap * LOG2E);
+#pragma unroll
+            for (int i = 0; i < 32; i++) s[i / 16][i % 16] = x[i];
 #pragma unroll
             for (int t = 0; t < 4; t++) { f[t] = 1.f; off[t] = 0.f; }
         }
@@ -633,7 +656,9 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
         }
 }
 
-// the splits of a tile joined: a thread takes four dimensions of one row
+// The splits of a tile joined.  Bound by the latency of its three dependent rounds of loads (which sequence, the partial
+// results, the sinks): a thread takes four dimensions of one row and asks for eight splits' numerators and sums at a time,
+// before it knows their maximum.
 template <class T, int R>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnLaunch a) {
     using V4 = typename Vec4<T>::type;
@@ -644,29 +669,45 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnLaunch a) {
     const int rows = min(R, n * a.group - tile * R);
     const int64_t size = R * (dp + 2);
     const float *part = a.part + ((int64_t)blockIdx.x * a.c.kv_heads + head) * a.splits * size;
-    for (int i = threadIdx.x; i < rows * quads; i += 256) {
+    for (int i = threadIdx.x + blockIdx.z * 256; i < rows * quads; i += 256 * gridDim.z) {
         const int row = i / quads, d = (i - row * quads) * 4;
         const int t = (tile * R + row) / a.group, h = head * a.group + tile * R + row - t * a.group;
-        float top = MINUS_INF;
-        for (int s = 0; s < a.splits; s++) top = fmaxf(top, part[s * size + R * dp + row]);
-        const float sink = a.sinks ? a.sinks[h] * LOG2E : MINUS_INF;
-        top = fmaxf(top, sink);
-        const float base = top == MINUS_INF ? 0.f : top;
-        float sum = 0.f;
+        float top = MINUS_INF, sum = 0.f;
         float4v y = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < a.splits; s++) {
-            const float l = part[s * size + R * dp + R + row];
-            if (l == 0.f) continue;  // a split that saw nothing
-            const float w = __builtin_amdgcn_exp2f(part[s * size + R * dp + row] - base);
-            const float4v x = *(const float4v *)(part + s * size + row * dp + d);
-            sum += l * w;
+        const float sink = a.sinks ? a.sinks[h] * LOG2E : MINUS_INF;
+        for (int s0 = 0; s0 < a.splits; s0 += 8) {
+            float m[8], l[8];
+            float4v x[8];
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] += x[e] * w;
+            for (int s = 0; s < 8; s++) {
+                const float *p = part + min(s0 + s, a.splits - 1) * size;
+                m[s] = p[R * dp + row];
+                l[s] = p[R * dp + R + row];
+                x[s] = *(const float4v *)(p + row * dp + d);
+            }
+            float best = top;
+#pragma unroll
+            for (int s = 0; s < 8; s++) best = fmaxf(best, m[s]);
+            const float base = best == MINUS_INF ? 0.f : best, keep = __builtin_amdgcn_exp2f(top - base);
+            top = best;
+            sum *= keep;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] *= keep;
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                if (s0 + s >= a.splits || l[s] == 0.f) continue;  // a split that saw nothing has no numerators
+                const float w = __builtin_amdgcn_exp2f(m[s] - base);
+                sum += l[s] * w;
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] += x[s][e] * w;
+            }
         }
-        const float total = sum + (a.sinks ? __builtin_amdgcn_exp2f(sink - base) : 0.f);
+        // the sink joins the sum; where it is the largest, everything is measured against it
+        const float all = fmaxf(top == MINUS_INF ? 0.f : top, sink), scale = __builtin_amdgcn_exp2f((top == MINUS_INF ? 0.f : top) - all);
+        const float total = sum * scale + (a.sinks ? __builtin_amdgcn_exp2f(sink - all) : 0.f);
         V4 w;
 #pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = (T)(sum == 0.f ? 0.f : y[e] / total);
+        for (int e = 0; e < 4; e++) w[e] = (T)(sum == 0.f ? 0.f : y[e] * scale / total);
         *(V4 *)((T *)a.out + (int64_t)(begin + t) * a.out_stride + (int64_t)h * a.c.head_dim + d) = w;
     }
 }
@@ -684,7 +725,8 @@ hipError_t launch_one(const AttnLaunch &a, hipStream_t s) {
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
-    attn_join_kernel<T, R><<<dim3((unsigned)a.items, (unsigned)a.c.kv_heads), 256, 0, s>>>(a);
+    // 256 threads take 8 rows of 128; a tile of 128 rows is given to 16 workgroups
+    attn_join_kernel<T, R><<<dim3((unsigned)a.items, (unsigned)a.c.kv_heads, R == ROWS ? 1 : 16), 256, 0, s>>>(a);
     return hipGetLastError();
 }
 

@@ -21,7 +21,7 @@ constexpr float PER127 = 0x1.020408p-7f;  // fl(1 / 127)
 // pages that the rows of sequence s touch, `first` their first token
 __device__ __forceinline__ int pages_touched(const DevBatch &b, int s, bool within_table, int &begin, int &n, int &first, int &len) {
     n = seq_rows(b, s, begin);
-    len = b.kv_len[s];
+    len = fixed(b.kv_len + s);
     first = len - n;
     if (n == 0 || len <= 0) return 0;
     int last = (len - 1) / KV_PAGE;
@@ -52,13 +52,14 @@ __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, cons
     if (!find_item(b.n_seqs, (int)blockIdx.x, [&](int s) { int x, y, z, w; return pages_touched(b, s, true, x, y, z, w); }, seq, local)) return;
     pages_touched(b, seq, true, begin, n, first, len);
     const int pi = max(first, 0) / KV_PAGE + local;
-    const int64_t phys = b.pages[(int64_t)seq * b.max_pages + pi];
-    if (phys < 0 || phys >= c.n_pages) return;
+    const int phys = fixed(b.pages + (int64_t)seq * b.max_pages + pi);
+    const bool there = phys >= 0 && phys < c.n_pages;
     const int t_lo = max(first - pi * KV_PAGE, 0), t_hi = min(len - pi * KV_PAGE, KV_PAGE);  // the page's new tokens
     const T *src = is_v ? xv : xk;
     const int64_t stride = is_v ? v_stride : k_stride;
     const int64_t row0 = (int64_t)begin + (pi * KV_PAGE - first);  // row of the page's token 0 (may lie before the sequence)
 
+    // the values first: they are asked for before it is known which page they go to
     float x[16][VEC];
     const bool live = lane * VEC < c.head_dim;
 #pragma unroll
@@ -73,7 +74,8 @@ __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, cons
                 if (live && lane * VEC + v < c.head_dim) x[j][v] = to_f32(p[v]);
         }
     }
-    const int64_t at = (phys * c.kv_heads + head);
+    if (!there) return;
+    const int64_t at = (int64_t)phys * c.kv_heads + head;
     float *scales = (is_v ? c.vs : c.ks) + at * c.per;
     uint8_t *codes = (is_v ? c.v : c.k) + at * (KV_PAGE * DP);
     const int going_on = t_lo % c.block ? t_lo / c.block : -1;  // the block that holds older tokens
@@ -131,25 +133,29 @@ __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, cons
         for (int v = 0; v < VEC; v++) {
             const int d = lane * VEC + v;
             if (d >= c.head_dim) continue;
-            uint4 *piece = (uint4 *)(codes + (((d / 16) * 4 + g) * 16 + d % 16) * 16);
+            uint8_t *piece = codes + (((d / 16) * 4 + g) * 16 + d % 16) * 16;
             uint32_t w[4];
-            if (!all) *(uint4 *)w = *piece;
+            if (moves) {
+                *(uint4 *)w = *(const uint4 *)piece;
 #pragma unroll
-            for (int m = 0; m < 4; m++) {
-                uint32_t r = 0;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int t = 16 * m + 4 * g + i;
-                    uint32_t byte = (uint32_t)q[4 * m + i][v];
-                    if (!all && !(t >= t_lo && t < t_hi)) {
-                        byte = w[m] >> (8 * i) & 0xff;
-                        if (t >= moved_lo && t < t_lo) byte = (uint32_t)(code_of((float)((int)byte - 128) * grown) + 128);
-                    }
-                    r |= byte << (8 * i);
+                for (int j = 0; j < 16; j++) {
+                    const int t = 16 * (j / 4) + 4 * g + j % 4;
+                    const int byte = (int)(w[j / 4] >> (8 * (j % 4)) & 0xff) - 128;
+                    if (t >= moved_lo && t < t_lo) piece[j] = (uint8_t)(code_of((float)byte * grown) + 128);
                 }
-                w[m] = r;
             }
-            *piece = *(uint4 *)w;
+            if (all) {
+#pragma unroll
+                for (int m = 0; m < 4; m++)
+                    w[m] = (uint32_t)q[4 * m][v] | (uint32_t)q[4 * m + 1][v] << 8 | (uint32_t)q[4 * m + 2][v] << 16 | (uint32_t)q[4 * m + 3][v] << 24;
+                *(uint4 *)piece = *(const uint4 *)w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const int t = 16 * (j / 4) + 4 * g + j % 4;
+                    if (t >= t_lo && t < t_hi) piece[j] = (uint8_t)q[j][v];
+                }
+            }
         }
         return;
     }
@@ -192,14 +198,14 @@ __global__ __launch_bounds__(256) void kv_read_kernel(DevKv c, DevBatch b, T *yk
     if (!find_item(b.n_seqs, (int)blockIdx.x, [&](int s) { int x, y, z, w; return pages_touched(b, s, false, x, y, z, w); }, seq, local)) return;
     pages_touched(b, seq, false, begin, n, first, len);
     const int pi = max(first, 0) / KV_PAGE + local;
-    int64_t phys = pi < b.max_pages ? b.pages[(int64_t)seq * b.max_pages + pi] : -1;
+    int phys = pi < b.max_pages ? fixed(b.pages + (int64_t)seq * b.max_pages + pi) : -1;
     const bool bad = phys < 0 || phys >= c.n_pages;  // such a page's tokens read as NaN
     if (bad) phys = 0;
     const int t_lo = max(first - pi * KV_PAGE, 0), t_hi = min(len - pi * KV_PAGE, KV_PAGE);
     T *dst = is_v ? yv : yk;
     const int64_t stride = is_v ? v_stride : k_stride;
     const int64_t row0 = (int64_t)begin + (pi * KV_PAGE - first);
-    const int64_t at = phys * c.kv_heads + head;
+    const int64_t at = (int64_t)phys * c.kv_heads + head;
     const float *scales = (is_v ? c.vs : c.ks) + at * c.per;
     const uint8_t *codes = (is_v ? c.v : c.k) + at * (KV_PAGE * DP);
     float s[4];
