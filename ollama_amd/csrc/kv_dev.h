@@ -47,6 +47,23 @@ __device__ __forceinline__ int seq_rows(const DevBatch &b, int s, int &begin) {
     return begin >= 0 && end <= b.n_rows && end > begin ? end - begin : 0;
 }
 
+// x of the lane that the data-parallel-primitive control names, 0 where there is none or its row of 16 lanes is masked out
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ int lane_of(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, CTRL, ROW_MASK, 0xf, true);
+}
+
+// sum over the lanes up to and with the own one: shifts by 1, 2, 4, 8 inside rows of 16, then row totals to the rows after
+__device__ __forceinline__ int scan_add(int x) {
+    x += lane_of<0x111>(x);
+    x += lane_of<0x112>(x);
+    x += lane_of<0x114>(x);
+    x += lane_of<0x118>(x);
+    x += lane_of<0x142, 0xa>(x);
+    x += lane_of<0x143, 0xc>(x);
+    return x;
+}
+
 // Work items numbered through the sequences, count(s) of them in sequence s: which sequence item `item` falls into and
 // its number there.  All lanes of a wave call it together; one round of loads per 64 sequences.
 template <class F>
@@ -56,12 +73,7 @@ __device__ __forceinline__ bool find_item(int n_seqs, int item, F count, int &se
     for (int s0 = 0; s0 < n_seqs; s0 += 64) {
         const int s = s0 + lane;
         const int c = s < n_seqs ? count(s) : 0;
-        int incl = c;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(incl, o);
-            if (lane >= o) incl += v;
-        }
+        const int incl = scan_add(c);
         const int total = __builtin_amdgcn_readlane(incl, 63);
         if (item < base + total) {
             const unsigned long long past = __ballot(base + incl > item);

@@ -29,15 +29,39 @@ __device__ __forceinline__ int pages_touched(const DevBatch &b, int s, bool with
     return max(0, last - max(first, 0) / KV_PAGE + 1);
 }
 
+// the largest of the wave's values, in lane 63
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+    v = max(v, (uint32_t)lane_of<0x111>((int)v));
+    v = max(v, (uint32_t)lane_of<0x112>((int)v));
+    v = max(v, (uint32_t)lane_of<0x114>((int)v));
+    v = max(v, (uint32_t)lane_of<0x118>((int)v));
+    v = max(v, (uint32_t)lane_of<0x142, 0xa>((int)v));
+    v = max(v, (uint32_t)lane_of<0x143, 0xc>((int)v));
     return v;
 }
 
-__device__ __forceinline__ int code_of(float x) {  // x already divided by the scale
-    const float r = rintf(x);
-    return (int)fminf(fmaxf(r, -127.f), 127.f);
+__device__ __forceinline__ int clamp_code(float r) { return (int)fminf(fmaxf(r, -127.f), 127.f); }
+
+// round(x / s) of the fp32 quotient, for N values.  x * (1 / s) is within 4e-5 of the quotient (127 and two roundings), so
+// its nearest whole number is the quotient's unless it lies that close to a half: then, and for scales whose reciprocal is
+// not safe, the division itself -- a tenth of the instructions otherwise.
+template <int N>
+__device__ __forceinline__ void codes_of(const float (&x)[N], float s, int (&q)[N]) {
+    const float inv = 1.0f / s;
+    float r[N];
+    bool sure = s >= 0x1p-100f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const float y = x[i] * inv;
+        r[i] = rintf(y);
+        sure = sure && fabsf(y - r[i]) < 0.4999f;
+    }
+    if (__ballot(!sure)) {
+#pragma unroll
+        for (int i = 0; i < N; i++) r[i] = s > 0.f ? rintf(x[i] / s) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) q[i] = clamp_code(r[i]) + 128;
 }
 
 template <class T, int VEC>
@@ -88,7 +112,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, cons
 #pragma unroll
             for (int v = 0; v < VEC; v++) big = max(big, __float_as_uint(x[j][v]) & 0x7fffffffu);
         big = wave_umax(big);
-        if (lane == 0) largest[g][m] = big;
+        if (lane == 63) largest[g][m] = big;
     }
     __syncthreads();
     float s[4], grown = 0.f;  // scale of the block that 16 tokens belong to; old scale / new scale where older codes move
@@ -116,9 +140,10 @@ __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, cons
 
     int q[16][VEC];
 #pragma unroll
-    for (int j = 0; j < 16; j++)
-#pragma unroll
-        for (int v = 0; v < VEC; v++) q[j][v] = s[j / 4] > 0.f ? code_of(x[j][v] / s[j / 4]) + 128 : 128;
+    for (int j = 0; j < 16; j++) {
+        const int t = 16 * (j / 4) + 4 * g + j % 4;
+        if (t >= t_lo && t < t_hi) codes_of(x[j], s[j / 4], q[j]);
+    }
 
     if (is_v) {
         bool any = false, all = true;
@@ -141,7 +166,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, cons
                 for (int j = 0; j < 16; j++) {
                     const int t = 16 * (j / 4) + 4 * g + j % 4;
                     const int byte = (int)(w[j / 4] >> (8 * (j % 4)) & 0xff) - 128;
-                    if (t >= moved_lo && t < t_lo) piece[j] = (uint8_t)(code_of((float)byte * grown) + 128);
+                    if (t >= moved_lo && t < t_lo) piece[j] = (uint8_t)(clamp_code(rintf((float)byte * grown)) + 128);
                 }
             }
             if (all) {
@@ -162,8 +187,10 @@ __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, cons
 #pragma unroll
     for (int j = 0; j < 16; j++) {
         const int t = 16 * (j / 4) + 4 * g + j % 4;
+        if (t >= t_lo && t < t_hi) {
 #pragma unroll
-        for (int v = 0; v < VEC; v++) tile[t * PITCH + lane * VEC + v] = (uint8_t)q[j][v];
+            for (int v = 0; v < VEC; v++) tile[t * PITCH + lane * VEC + v] = (uint8_t)q[j][v];
+        }
     }
     __syncthreads();
 #pragma unroll
@@ -179,7 +206,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, cons
             for (int m = 0; m < 4; m++) {
                 uint32_t r = 0;
 #pragma unroll
-                for (int i = 0; i < 4; i++) r |= (uint32_t)(code_of((float)((int)(w[m] >> (8 * i) & 0xff) - 128) * grown) + 128) << (8 * i);
+                for (int i = 0; i < 4; i++) r |= (uint32_t)(clamp_code(rintf((float)((int)(w[m] >> (8 * i) & 0xff) - 128) * grown)) + 128) << (8 * i);
                 w[m] = r;
             }
             *piece = *(uint4 *)w;
@@ -221,8 +248,16 @@ __global__ __launch_bounds__(256) void kv_read_kernel(DevKv c, DevBatch b, T *yk
         } else {
             const int d = i / 64 * 16 + i % 16, g = i % 64 / 16;
             const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+            // four lanes hold four tokens of four dimensions: turned over, each has four dimensions of one token
+            const int u = tid & 3;
 #pragma unroll
-            for (int j = 0; j < 16; j++) tile[(16 * (j / 4) + 4 * g + j % 4) * PITCH + d] = (uint8_t)(ws[j / 4] >> (8 * (j % 4)));
+            for (int m = 0; m < 4; m++) {
+                const uint32_t b1 = (uint32_t)lane_of<0xB1>((int)ws[m]);  // of lane ^ 1
+                const uint32_t a = u & 1 ? __builtin_amdgcn_perm(ws[m], b1, 0x07030501u) : __builtin_amdgcn_perm(b1, ws[m], 0x06020400u);
+                const uint32_t b2 = (uint32_t)lane_of<0x4E>((int)a);      // of lane ^ 2
+                const uint32_t r = u & 2 ? __builtin_amdgcn_perm(a, b2, 0x07060302u) : __builtin_amdgcn_perm(b2, a, 0x05040100u);
+                *(uint32_t *)(tile + (16 * m + 4 * g + u) * PITCH + d - u) = r;
+            }
         }
     }
     __syncthreads();
