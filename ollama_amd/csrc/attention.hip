@@ -30,8 +30,6 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 
 typedef float float16v __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(1))) const void glb_ptr_t;
-typedef __attribute__((address_space(3))) void lds_ptr_t;
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float MINUS_INF = -__builtin_inff();
@@ -132,21 +130,61 @@ __device__ __forceinline__ void cap_scores(float (&x)[N], float c) {
 // a / b where both are the same for the whole wave (a division is vector code: its result goes back to a scalar register)
 __device__ __forceinline__ int same(int a, int b) { return __builtin_amdgcn_readfirstlane(a / b); }
 
-// the page that holds tokens 64 page .. 64 page + 63 of sequence seq; -1: there is none
-__device__ __forceinline__ int page_of(const AttnLaunch &a, int seq, int page) {
-    const int phys = page < a.b.max_pages ? fixed(a.b.pages + (int64_t)seq * a.b.max_pages + page) : -1;
-    return phys < a.c.n_pages ? phys : -1;
+// Numbers of a sequence's pages, 64 at a time in the lanes of a register: pages from + step * (0 .. 63).  Neither they nor
+// the scales go through scalar loads: those share their counter with LDS reads and come back in any order, so every LDS
+// read behind one would wait for the cache's memory.
+__device__ __forceinline__ int pages_from(const AttnLaunch &a, int seq, int from, int step) {
+    const int page = from + step * (int)(threadIdx.x & 63);
+    const int phys = page < a.b.max_pages ? a.b.pages[(int64_t)seq * a.b.max_pages + page] : -1;
+    return phys < a.c.n_pages ? phys : -1;  // -1: there is no such page
 }
 
-// the scales of its groups of 16 tokens; NaN where there is no such page: whoever sees it gets NaN
-__device__ __forceinline__ void scales_of(const AttnLaunch &a, int64_t at, bool bad, float (&ks)[4], float (&vs)[4]) {
+// the scales of a page's four groups of 16 tokens: keys' in lanes 0 .. 3 (of every 8), values' in lanes 4 .. 7
+__device__ __forceinline__ float scales_from(const AttnLaunch &a, int phys, int head) {
+    const int64_t i = ((int64_t)max(phys, 0) * a.c.kv_heads + head) * a.c.per + ((threadIdx.x & 3) >> a.shift);
+    return threadIdx.x & 4 ? a.c.vs[i] : a.c.ks[i];
+}
+
+__device__ __forceinline__ float lane_float(float x, int lane) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), lane));
+}
+
+// as scalars; NaN where there is no such page: whoever sees it gets NaN
+__device__ __forceinline__ void spread_scales(float x, int phys, float (&ks)[4], float (&vs)[4]) {
+    x = phys < 0 ? __builtin_nanf("") : x;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-        const int64_t i = at * a.c.per + (t >> a.shift);
-        const float k = fixed(a.c.ks + i), v = fixed(a.c.vs + i);
-        ks[t] = bad ? __builtin_nanf("") : k;
-        vs[t] = bad ? __builtin_nanf("") : v;
+        ks[t] = lane_float(x, t);
+        vs[t] = lane_float(x, 4 + t);
     }
+}
+
+// A barrier for what the waves put into LDS alone: __syncthreads() would also wait for the loads of the page after next.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// x in a register of its own, copied here.  A register that a load of the loop's next round writes must not be handed on or
+// changed in place: the compiler then copies it at the end of the round, where that waits for the load just issued.
+__device__ __forceinline__ uint32_t copied(uint32_t x) {
+    uint32_t y;
+    asm("v_mov_b32 %0, %1" : "=v"(y) : "v"(x));
+    return y;
+}
+
+// The order of N LDS reads and their PER matrix instructions each: four reads ahead of the instructions.  Left to itself the
+// compiler puts two reads right in front of the two instructions that want them, and a wave waits for LDS every time.
+template <int N, int PER>
+__device__ __forceinline__ void interleave() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < N - 4; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 4 * PER, 0);
 }
 
 // Scales that are no numbers (a poisoned block, a page that there is not) are taken out of a page's work -- masked tokens of
@@ -248,9 +286,12 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
         t0 = t0 + (int)blockIdx.z * share;
         t1 = min(t1, t0 + share);
     }
-    for (int page = t0 + wave; page < t1; page += 4) {
-        const int phys = page_of(a, seq, page);
+    int ids = 0;
+    for (int page = t0 + wave, k = 0; page < t1; page += 4, k++) {
+        if (k % 64 == 0) ids = pages_from(a, seq, page, 4);
+        const int phys = __builtin_amdgcn_readlane(ids, k % 64);
         const int64_t at = (int64_t)max(phys, 0) * a.c.kv_heads + head;
+        const float sc = scales_from(a, phys, head);
         const uint4 *kp = (const uint4 *)(a.c.k + at * (KV_PAGE * DP)) + lane;
         const uint4 *vp = (const uint4 *)(a.c.v + at * (KV_PAGE * DP)) + lane;
         uint4 kc[4][NC], vc[4 * NC];
@@ -261,7 +302,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
 #pragma unroll
         for (int d = 0; d < 4 * NC; d++) vc[d] = vp[d * 64];
         float ks[4], vs[4];
-        scales_of(a, at, phys < 0, ks, vs);
+        spread_scales(sc, phys, ks, vs);
         const int j0 = page * KV_PAGE;
         take_out_nan(ks, vs, j0, lo, hi, l);
         float z[16];
@@ -417,7 +458,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
     constexpr bool PHILO = !__is_same(T, __bf16);      // probabilities in two halves
     constexpr int DP = 64 * NC, BYTES = KV_PAGE * DP;  // of a page's keys (and values) of one head
     using V4 = typename Vec4<T>::type;
-    __shared__ __align__(1024) uint8_t buf[2][2 * BYTES];
+    extern __shared__ __align__(1024) uint8_t lds[];  // two buffers of a page's keys and values as halves
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const int r = lane % 32, h = lane / 32;
     // heads fastest: with eight of them every XCD keeps one head's cache in its L2; later tiles (longer ones) first
@@ -489,23 +530,54 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
         t0 = t0 + (int)blockIdx.z * share;
         t1 = min(t1, t0 + share);
     }
+    // A wave's share of a page: codes of 16 tokens (its number) of every 64 dimensions, and NC pieces of 16 dimensions of all
+    // tokens; asked for one page ahead, widened and put into LDS in the order the matrix instructions take them.
+    uint4 kc[NC], vc[NC];
     float ks[4], vs[4];
-    auto fetch = [&](int phys, int b) {
+    auto fetch = [&](int phys) {
         const int64_t at = (int64_t)max(phys, 0) * a.c.kv_heads + head;
+        const uint4 *kp = (const uint4 *)(a.c.k + at * BYTES) + wave * NC * 64 + lane, *vp = (const uint4 *)(a.c.v + at * BYTES) + wave * NC * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < NC; i++) { kc[i] = kp[i * 64]; vc[i] = vp[i * 64]; }
+    };
+    auto place = [&](int b) {
+        uint8_t *kb = lds + b * 4 * BYTES, *vb = kb + 2 * BYTES;
+        const int g = lane / 16, x = lane % 16;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            uint8_t *p = kb + (((wave / 2 * NC + c) * 2 + g / 2) * 2) * 1024 + ((g & 1) * 32 + (wave & 1) * 16 + x) * 16;
+            *(half8 *)p = HILO ? widen_centred(kc[c].x, kc[c].y) : widen(kc[c].x, kc[c].y);
+            *(half8 *)(p + 1024) = HILO ? widen_centred(kc[c].z, kc[c].w) : widen(kc[c].z, kc[c].w);
+        }
 #pragma unroll
         for (int i = 0; i < NC; i++) {
-            const int kb = (wave * NC + i) * 1024;
-            __builtin_amdgcn_global_load_lds((glb_ptr_t *)(a.c.k + at * BYTES + kb + lane * 16), (lds_ptr_t *)(buf[b] + kb), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((glb_ptr_t *)(a.c.v + at * BYTES + kb + lane * 16), (lds_ptr_t *)(buf[b] + BYTES + kb), 16, 0, 0);
+            const int dt = wave * NC + i;
+            // lanes 32 apart hold tokens 4 g .. and 4 (g + 2) .. of each 16: exchanged, each has both of two sixteens
+            const auto s0 = __builtin_amdgcn_permlane32_swap(copied(vc[i].x), copied(vc[i].z), false, false);
+            const auto s1 = __builtin_amdgcn_permlane32_swap(copied(vc[i].y), copied(vc[i].w), false, false);
+            uint8_t *p = vb + (dt / 2 * 4 + lane / 32 * 2) * 1024 + ((g & 1) * 32 + (dt & 1) * 16 + x) * 16;
+            *(half8 *)p = widen_centred(s0[0], s0[1]);
+            *(half8 *)(p + 1024) = widen_centred(s1[0], s1[1]);
         }
-        scales_of(a, at, phys < 0, ks, vs);
     };
-    // a page's number two pages ahead of its use: the number, then its codes and scales, then the work
-    if (t0 < t1) fetch(page_of(a, seq, t0), 0);
-    int next = page_of(a, seq, t0 + 1);
+    // this page's, the next one's and the one after's number; scales of the first two
+    int ids = pages_from(a, seq, t0, 1);
+    int phys = __builtin_amdgcn_readlane(ids, 0), next = __builtin_amdgcn_readlane(ids, 1);
+    float sc = 0.f, next_sc = 0.f;
+    if (t0 < t1) {
+        sc = scales_from(a, phys, head);
+        fetch(phys);
+        place(0);
+        next_sc = scales_from(a, next, head);
+        fetch(next);
+    }
     for (int page = t0; page < t1; page++) {
         const int b = (page - t0) & 1;
+        lds_barrier();
+        spread_scales(sc, phys, ks, vs);
         const int j0 = page * KV_PAGE;
+        const bool works = wrow0 < rows && j0 < w_hi_max && j0 + KV_PAGE > w_lo_min;  // else nothing that this wave's rows see
+        if (works) {
         take_out_nan(ks, vs, j0, lo, hi, l);
         float f[4], w[4], off[4];  // a score is s * f + off
         const float vmax = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
@@ -516,34 +588,24 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
             off[t] = HILO ? 0.f : minus_bias * f[t];
             w[t] = vs[t];
         }
-        __builtin_amdgcn_s_waitcnt((0 & 15) | (7 << 4) | (15 << 8));  // vmcnt(0): this wave's part of the page is in LDS
-        __syncthreads();
-        if (page + 1 < t1) {
-            fetch(next, b ^ 1);
-            next = page_of(a, seq, page + 2);
-        }
-        if (wrow0 >= rows || j0 >= w_hi_max || j0 + KV_PAGE <= w_lo_min) continue;  // nothing that this wave's rows see
-        const uint8_t *kb = buf[b], *vb = buf[b] + BYTES;
-        float16v s[2];
+        const half8 *kb = (const half8 *)(lds + b * 4 * BYTES) + lane, *vb = kb + 2 * BYTES / 16;
+        // two accumulators in turn: a matrix instruction that continues the one right before it waits for it
+        float16v s[2] = {float16v{}, float16v{}};
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
+        for (int c = 0; c < NC; c++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[t][i] = 0.f;
+            for (int e = 0; e < 2; e++)
 #pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const uint4 x = *(const uint4 *)(kb + (((2 * t + r / 16) * NC + c) * 64 + (2 * e + h) * 16 + r % 16) * 16);
-                    const half8 k0 = HILO ? widen_centred(x.x, x.y) : widen(x.x, x.y);
-                    const half8 k1 = HILO ? widen_centred(x.z, x.w) : widen(x.z, x.w);
-                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qh[c][e][0].v, s[t], 0, 0, 0);
-                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[c][e][1].v, s[t], 0, 0, 0);
+                for (int i = 0; i < 2; i++) {
+                    const half8 k0 = kb[((c * 2 + e) * 2 + i) * 64], k1 = kb[(((NC + c) * 2 + e) * 2 + i) * 64];
+                    s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qh[c][e][i].v, s[0], 0, 0, 0);
+                    s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[c][e][i].v, s[1], 0, 0, 0);
                     if (HILO) {
-                        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[HILO ? c : 0][e][0].v, s[t], 0, 0, 0);
-                        s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[HILO ? c : 0][e][1].v, s[t], 0, 0, 0);
+                        s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[HILO ? c : 0][e][i].v, s[0], 0, 0, 0);
+                        s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[HILO ? c : 0][e][i].v, s[1], 0, 0, 0);
                     }
                 }
-        }
+        interleave<8 * NC, HILO ? 2 : 1>();
         if (CAP) {
             float x[32];
 #pragma unroll
@@ -603,17 +665,26 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
             }
         }
 #pragma unroll
-        for (int d = 0; d < 2 * NC; d++) {
-            const uint4 x0 = *(const uint4 *)(vb + ((2 * d + r / 16) * 64 + h * 16 + r % 16) * 16);
-            const uint4 x1 = *(const uint4 *)(vb + ((2 * d + r / 16) * 64 + (h + 2) * 16 + r % 16) * 16);
-            const uint32_t a0[4] = {x0.x, x0.y, x0.z, x0.w}, a1[4] = {x1.x, x1.y, x1.z, x1.w};
+        for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const half8 v = widen_centred(a0[t], a1[t]);
+            for (int d = 0; d < 2 * NC; d++) {
+                const half8 v = vb[(d * 4 + t) * 64];
                 acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[t].v, acc[d], 0, 0, 0);
                 if (PHILO) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[PHILO ? t : 0].v, acc[d], 0, 0, 0);
             }
+        interleave<8 * NC, PHILO ? 2 : 1>();
         }
+        // The next page into the other buffer, which every wave left before this page's barrier.  Behind the last page this
+        // goes on with pages that nobody works on (their number is the table's, or none: then page 0): without a condition
+        // the loads go straight into the registers that the next round reads, with one they are waited for here.
+        place(b ^ 1);
+        sc = __uint_as_float(copied(__float_as_uint(next_sc)));
+        phys = next;
+        const int k = page + 2 - t0;
+        if (k % 64 == 0) ids = pages_from(a, seq, page + 2, 1);
+        next = __builtin_amdgcn_readlane(ids, k % 64);
+        next_sc = scales_from(a, next, head);
+        fetch(next);
     }
 
     l += __shfl_xor(l, 32);
@@ -720,8 +791,10 @@ hipError_t launch_one(const AttnLaunch &a, hipStream_t s) {
         else attn_rows_kernel<T, NC, false><<<grid, 256, 0, s>>>(a);
     } else {
         const dim3 grid((unsigned)a.items * (unsigned)a.c.kv_heads, 1, (unsigned)a.splits);
-        if (a.softcap > 0.f) attn_tile_kernel<T, NC, true><<<grid, 256, 0, s>>>(a);
-        else attn_tile_kernel<T, NC, false><<<grid, 256, 0, s>>>(a);
+        const auto kernel = a.softcap > 0.f ? attn_tile_kernel<T, NC, true> : attn_tile_kernel<T, NC, false>;
+        constexpr int lds = 2 * 4 * KV_PAGE * 64 * NC;
+        if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        kernel<<<grid, 256, lds, s>>>(a);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
