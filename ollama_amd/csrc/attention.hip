@@ -451,6 +451,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
 // rows at a head of 128 the matrix cores have 1024 cycles of work; widening the codes and the softmax of 2048 scores, a
 // quarter-rate exponential each, are about twice that.
 constexpr int TILE = 128;
+constexpr float LAZY = 6.f;
 
 template <class T, int NC, bool CAP>
 __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLaunch a) {
@@ -522,7 +523,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
     float m = MINUS_INF, l = 0.f;
-    float ref = 0x1p-100f, unit = 0x1p115f;  // values are accumulated in units of ref * 2^-15 = 1 / unit
+    float ref = 0x1p-100f, unit = 0x1p109f;  // values are accumulated in units of ref * 2^-9 = 1 / unit
 
     int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
     if (a.splits > 1) {
@@ -580,7 +581,6 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
         if (works) {
         take_out_nan(ks, vs, j0, lo, hi, l);
         float f[4], w[4], off[4];  // a score is s * f + off
-        const float vmax = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             f[t] = score_scale * ks[t];
@@ -631,39 +631,74 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
             for (int i = 1; i < 8; i++) x = fmaxf(x, s[t / 2][8 * (t % 2) + i]);
             top = fmaxf(top, __builtin_fmaf(x, f[t], off[t]));
         }
+        // The row's reference follows its maximum only when that has left it 2^6 behind: among 32 rows one has a new maximum
+        // on almost every page, and each time the accumulators are rescaled.  Probabilities are then up to 2^6, and halves
+        // hold them times 2^9.
+        const float vmax = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float m_new = fmaxf(m, top), base = m_new == MINUS_INF ? 0.f : m_new;
-        float keep = __builtin_amdgcn_exp2f(m - base);
-        l *= keep;
-        if (vmax > ref) {
-            const int e = min(exponent(vmax) + 1, 126);
-            keep *= ref * pow2(-e);
-            ref = pow2(e);
-            unit = e >= -100 ? pow2(15 - e) : unit;
-        }
-        m = m_new;
-        if (__ballot(keep != 1.f)) {
+        const bool larger = vmax > ref;  // the same for all lanes
+        if (__ballot(top > m + LAZY) || larger) {
+            const float m_new = fmaxf(m, top);
+            float keep = __builtin_amdgcn_exp2f(m - (m_new == MINUS_INF ? 0.f : m_new));
+            l *= keep;
+            if (larger) {
+                const int e = min(exponent(vmax) + 1, 126);
+                keep *= ref * pow2(-e);
+                ref = pow2(e);
+                unit = e >= -100 ? pow2(9 - e) : unit;
+            }
+            m = m_new;
 #pragma unroll
             for (int d = 0; d < 2 * NC; d++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) acc[d][i] *= keep;
         }
+        const float base = m == MINUS_INF ? 0.f : m;
         Halves ph[4], pl[PHILO ? 4 : 1];
+        // 16-bit calls: the value scale goes into the exponent and the sum of the probabilities comes back from the weighted
+        // ones -- while no scale is so far below the largest that halves would lose the sum.  A block of zeros may have any
+        // scale.  Logarithm and reciprocal of the page's scales are taken once, in the lanes that hold them.
+        const float wl = sc == 0.f ? ref * unit : sc * unit;
+        if (!HILO && __ballot((lane & 4) && !(wl >= 0x1p-3f)) == 0) {
+            const float log_w = __builtin_amdgcn_logf(wl), inv_w = __builtin_amdgcn_rcpf(wl);
+            const half2v ones = {(_Float16)1.f, (_Float16)1.f};
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const float wt = w[t] * unit, shift = off[t] - base;
+            for (int t = 0; t < 4; t++) {
+                const float shift = off[t] - base + lane_float(log_w, 4 + t);
+                float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float z = s[t / 2][8 * (t % 2) + i];
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z, f[t], shift));
-                l += p;
-                float y = p * wt;
-                if (PHILO) y = settled(y);
-                const _Float16 x = (_Float16)y;
-                ph[t].v[i] = x;
-                if (PHILO) pl[PHILO ? t : 0].v[i] = (_Float16)(y - (float)x);
+                for (int i = 0; i < 8; i += 2) {
+                    const float y0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][8 * (t % 2) + i], f[t], shift));
+                    const float y1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][8 * (t % 2) + i + 1], f[t], shift));
+                    const half2v x = {(_Float16)y0, (_Float16)y1};
+                    ph[t].h[i / 2] = x;
+                    if (PHILO) {
+                        const half2v rest = {(_Float16)(y0 - (float)x[0]), (_Float16)(y1 - (float)x[1])};
+                        pl[PHILO ? t : 0].h[i / 2] = rest;
+                        sum += y0 + y1;
+                    } else {
+                        sum = __builtin_amdgcn_fdot2(x, ones, sum, false);
+                    }
+                }
+                l = __builtin_fmaf(sum, lane_float(inv_w, 4 + t), l);
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const float wt = w[t] * unit, shift = off[t] - base;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t / 2][8 * (t % 2) + i], f[t], shift));
+                    l += p;
+                    float y = p * wt;
+                    if (PHILO) y = settled(y);
+                    const _Float16 x = (_Float16)y;
+                    ph[t].v[i] = x;
+                    if (PHILO) pl[PHILO ? t : 0].v[i] = (_Float16)(y - (float)x);
+                }
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -691,7 +726,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
     if (!valid) return;
     const int o_h = head * a.group + my_h;
     const float base = m == MINUS_INF ? 0.f : m;
-    float weight = ref * 0x1p-15f;
+    float weight = ref * 0x1p-9f;
     float *part = a.part + (((int64_t)item * a.c.kv_heads + head) * a.splits + blockIdx.z) * (TILE * (DP + 2));
     const int in_tile = 32 * wave + r;
     if (a.splits == 1) {
