@@ -89,12 +89,17 @@ __device__ __forceinline__ float settled(float x) {
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
 __device__ __forceinline__ int exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 0xff) - 127; }
 
-// tiles of R rows that this launch has in sequence s
+// tiles of R rows that this launch has in a sequence of n rows
 template <int R>
-__device__ __forceinline__ int tiles_of(const AttnLaunch &a, int s) {
-    int begin;
-    const int rows = seq_rows(a.b, s, begin) * a.group;
+__device__ __forceinline__ int tiles_of(const AttnLaunch &a, int n) {
+    const int rows = n * a.group;
     return rows >= a.least && rows <= a.most ? (rows + R - 1) / R : 0;
+}
+
+// the value of the lane 32 away, exchanged in the registers
+__device__ __forceinline__ float other_half(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(threadIdx.x & 32 ? r[0] : r[1]);
 }
 
 __device__ __forceinline__ void visible(const AttnLaunch &a, int pos, int len, int &lo, int &hi) {
@@ -218,10 +223,10 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const int r = lane % 16, g = lane / 16;
     const int head = blockIdx.y;  // key/value head
-    int seq, tile;
-    if (!find_item(a.b.n_seqs, (int)blockIdx.x, [&](int s) { return tiles_of<ROWS>(a, s); }, seq, tile)) return;
-    int begin;
-    const int n = seq_rows(a.b, seq, begin), len = fixed(a.b.kv_len + seq), first = len - n;
+    Found at_item;
+    if (!find_item(a.b, (int)blockIdx.x, [&](int n, int) { return tiles_of<ROWS>(a, n); }, at_item)) return;
+    const int seq = at_item.seq, tile = at_item.local, begin = at_item.begin;
+    const int n = at_item.n, len = at_item.len, first = len - n;
     const int rows = n * a.group, row0 = tile * ROWS;
     const bool valid = row0 + r < rows;
     const int my_t = valid ? (row0 + r) / a.group : 0, my_h = valid ? row0 + r - my_t * a.group : 0;
@@ -464,10 +469,10 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
     const int r = lane % 32, h = lane / 32;
     // heads fastest: with eight of them every XCD keeps one head's cache in its L2; later tiles (longer ones) first
     const int head = blockIdx.x % a.c.kv_heads, item = a.items - 1 - (int)blockIdx.x / a.c.kv_heads;
-    int seq, tile;
-    if (!find_item(a.b.n_seqs, item, [&](int s) { return tiles_of<TILE>(a, s); }, seq, tile)) return;
-    int begin;
-    const int n = seq_rows(a.b, seq, begin), len = fixed(a.b.kv_len + seq), first = len - n;
+    Found at_item;
+    if (!find_item(a.b, item, [&](int n, int) { return tiles_of<TILE>(a, n); }, at_item)) return;
+    const int seq = at_item.seq, tile = at_item.local, begin = at_item.begin;
+    const int n = at_item.n, len = at_item.len, first = len - n;
     const int rows = n * a.group, row0 = tile * TILE, wrow0 = row0 + 32 * wave;
     const bool valid = wrow0 + r < rows;
     const int my_t = valid ? (wrow0 + r) / a.group : 0, my_h = valid ? wrow0 + r - my_t * a.group : 0;
@@ -478,58 +483,25 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
     visible(a, first + same(min(wrow0, rows - 1), a.group), len, w_lo_min, w_hi_min);
     visible(a, first + same(min(wrow0 + 32, rows) - 1, a.group), len, w_lo_max, w_hi_max);
 
-    // queries: dimensions 64 c + 16 (2 e + h) + 8 i .. + 7 of row r, as the second operand of step (c, e, i)
-    Halves qh[NC][2][2], ql[HILO ? NC : 1][2][2];
-    float score_scale, minus_bias;
+    // Everything that a tile waits for once is asked for as early as it can be: page numbers, queries, the first page.
+    int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
+    if (a.splits > 1) {
+        const int share = same(t1 - t0 + a.splits - 1, a.splits);
+        t0 = t0 + (int)blockIdx.z * share;
+        t1 = min(t1, t0 + share);
+    }
+    int ids = pages_from(a, seq, t0, 1);  // this page's, the next one's and the one after's number; scales of the first two
+    typename Vec4<T>::type raw[NC][8];
     {
-        float x[NC][2][16];
-        float big = 0.f;
         const T *p = (const T *)a.q + (int64_t)(begin + my_t) * a.q_stride + (int64_t)(head * a.group + my_h) * a.c.head_dim;
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int d = 64 * c + 16 * (2 * (i / 4) + h) + 4 * (i % 4);
-                V4 y = {};
-                if (valid && d < a.c.head_dim) y = *(const V4 *)(p + d);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    x[c][i / 4][4 * (i % 4) + e] = to_f32(y[e]);
-                    big = fmaxf(big, fabsf(to_f32(y[e])));
-                }
+                raw[c][i] = V4{};
+                if (valid && d < a.c.head_dim) raw[c][i] = *(const V4 *)(p + d);
             }
-        big = fmaxf(big, __shfl_xor(big, 32));
-        const int e = min(max(13 - exponent(big), -100), 100);
-        const float up = a.scale < 0.f ? -pow2(e) : pow2(e);  // the scale's sign goes into the queries
-        float sum = 0.f;
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int i = 0; i < 32; i++) {
-                const float y = x[c][i / 16][i % 16] * up;
-                const _Float16 z = (_Float16)y;
-                qh[c][i / 16][i / 8 % 2].v[i % 8] = z;
-                sum += (float)z;
-                if (HILO) ql[HILO ? c : 0][i / 16][i / 8 % 2].v[i % 8] = (_Float16)(y - (float)z);
-            }
-        sum += __shfl_xor(sum, 32);
-        minus_bias = HILO ? 0.f : sum * (-128.f * 0x1p-24f);
-        score_scale = fabsf(a.scale) * (HILO ? 1.f : 0x1p24f) * pow2(-e) * (CAP ? 1.f / a.softcap : LOG2E);
-    }
-
-    float16v acc[2 * NC];
-#pragma unroll
-    for (int d = 0; d < 2 * NC; d++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
-    float m = MINUS_INF, l = 0.f;
-    float ref = 0x1p-100f, unit = 0x1p109f;  // values are accumulated in units of ref * 2^-9 = 1 / unit
-
-    int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
-    if (a.splits > 1) {
-        const int share = same(t1 - t0 + a.splits - 1, a.splits);
-        t0 = t0 + (int)blockIdx.z * share;
-        t1 = min(t1, t0 + share);
     }
     // A wave's share of a page: codes of 16 tokens (its number) of every 64 dimensions, and NC pieces of 16 dimensions of all
     // tokens; asked for one page ahead, widened and put into LDS in the order the matrix instructions take them.
@@ -561,17 +533,55 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
             *(half8 *)(p + 1024) = widen_centred(s1[0], s1[1]);
         }
     };
-    // this page's, the next one's and the one after's number; scales of the first two
-    int ids = pages_from(a, seq, t0, 1);
     int phys = __builtin_amdgcn_readlane(ids, 0), next = __builtin_amdgcn_readlane(ids, 1);
-    float sc = 0.f, next_sc = 0.f;
-    if (t0 < t1) {
-        sc = scales_from(a, phys, head);
-        fetch(phys);
-        place(0);
-        next_sc = scales_from(a, next, head);
-        fetch(next);
+    float sc = scales_from(a, phys, head), next_sc = 0.f;
+    fetch(phys);
+
+    // queries: dimensions 64 c + 16 (2 e + h) + 8 i .. + 7 of row r, as the second operand of step (c, e, i)
+    Halves qh[NC][2][2], ql[HILO ? NC : 1][2][2];
+    float score_scale, minus_bias;
+    {
+        float x[NC][2][16];
+        float big = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    x[c][i / 4][4 * (i % 4) + e] = to_f32(raw[c][i][e]);
+                    big = fmaxf(big, fabsf(to_f32(raw[c][i][e])));
+                }
+        big = fmaxf(big, other_half(big));
+        const int e = min(max(13 - exponent(big), -100), 100);
+        const float up = a.scale < 0.f ? -pow2(e) : pow2(e);  // the scale's sign goes into the queries
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+                const float y = x[c][i / 16][i % 16] * up;
+                const _Float16 z = (_Float16)y;
+                qh[c][i / 16][i / 8 % 2].v[i % 8] = z;
+                sum += (float)z;
+                if (HILO) ql[HILO ? c : 0][i / 16][i / 8 % 2].v[i % 8] = (_Float16)(y - (float)z);
+            }
+        sum += other_half(sum);
+        minus_bias = HILO ? 0.f : sum * (-128.f * 0x1p-24f);
+        score_scale = fabsf(a.scale) * (HILO ? 1.f : 0x1p24f) * pow2(-e) * (CAP ? 1.f / a.softcap : LOG2E);
     }
+
+    place(0);
+    next_sc = scales_from(a, next, head);
+    fetch(next);
+    float16v acc[2 * NC];
+#pragma unroll
+    for (int d = 0; d < 2 * NC; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
+    float m = MINUS_INF, l = 0.f;
+    float ref = 0x1p-100f, unit = 0x1p109f;  // values are accumulated in units of ref * 2^-9 = 1 / unit
+
     for (int page = t0; page < t1; page++) {
         const int b = (page - t0) & 1;
         lds_barrier();
@@ -635,7 +645,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
         // on almost every page, and each time the accumulators are rescaled.  Probabilities are then up to 2^6, and halves
         // hold them times 2^9.
         const float vmax = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-        top = fmaxf(top, __shfl_xor(top, 32));
+        top = fmaxf(top, other_half(top));
         const bool larger = vmax > ref;  // the same for all lanes
         if (__ballot(top > m + LAZY) || larger) {
             const float m_new = fmaxf(m, top);
@@ -722,7 +732,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
         fetch(next);
     }
 
-    l += __shfl_xor(l, 32);
+    l += other_half(l);
     if (!valid) return;
     const int o_h = head * a.group + my_h;
     const float base = m == MINUS_INF ? 0.f : m;
@@ -769,9 +779,9 @@ template <class T, int R>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnLaunch a) {
     using V4 = typename Vec4<T>::type;
     const int head = blockIdx.y, dp = a.c.dp, quads = a.c.head_dim / 4;
-    int seq, tile, begin;
-    if (!find_item(a.b.n_seqs, (int)blockIdx.x, [&](int s) { return tiles_of<R>(a, s); }, seq, tile)) return;
-    const int n = seq_rows(a.b, seq, begin);
+    Found at_item;
+    if (!find_item(a.b, (int)blockIdx.x, [&](int n, int) { return tiles_of<R>(a, n); }, at_item)) return;
+    const int tile = at_item.local, begin = at_item.begin, n = at_item.n;
     const int rows = min(R, n * a.group - tile * R);
     const int64_t size = R * (dp + 2);
     const float *part = a.part + ((int64_t)blockIdx.x * a.c.kv_heads + head) * a.splits * size;

@@ -40,13 +40,6 @@ __device__ __forceinline__ T fixed(const T *p) {
     return *(const __attribute__((address_space(4))) T *)p;
 }
 
-// rows of sequence s and the first of them; a range that is no part of 0..n_rows counts as none
-__device__ __forceinline__ int seq_rows(const DevBatch &b, int s, int &begin) {
-    begin = fixed(b.row_start + s);
-    const int end = fixed(b.row_start + s + 1);
-    return begin >= 0 && end <= b.n_rows && end > begin ? end - begin : 0;
-}
-
 // x of the lane that the data-parallel-primitive control names, 0 where there is none or its row of 16 lanes is masked out
 template <int CTRL, int ROW_MASK = 0xf>
 __device__ __forceinline__ int lane_of(int x) {
@@ -64,22 +57,38 @@ __device__ __forceinline__ int scan_add(int x) {
     return x;
 }
 
-// Work items numbered through the sequences, count(s) of them in sequence s: which sequence item `item` falls into and
-// its number there.  All lanes of a wave call it together; one round of loads per 64 sequences.
+// where a work item falls: its sequence, its number there, and the sequence's rows
+struct Found {
+    int seq, local;
+    int begin, n, len;  // first row, rows, tokens
+};
+
+// Work items numbered through the sequences, count(n, len) of them in a sequence of n rows and len tokens: where item
+// `item` falls.  A row range that is no part of 0..n_rows counts as none.  All lanes of a wave call it together; one round
+// of loads per 64 sequences.
 template <class F>
-__device__ __forceinline__ bool find_item(int n_seqs, int item, F count, int &seq, int &local) {
+__device__ __forceinline__ bool find_item(const DevBatch &b, int item, F count, Found &f) {
     const int lane = threadIdx.x & 63;
     int base = 0;
-    for (int s0 = 0; s0 < n_seqs; s0 += 64) {
+    for (int s0 = 0; s0 < b.n_seqs; s0 += 64) {
         const int s = s0 + lane;
-        const int c = s < n_seqs ? count(s) : 0;
+        int begin = 0, n = 0, len = 0, c = 0;
+        if (s < b.n_seqs) {
+            begin = b.row_start[s];
+            const int end = b.row_start[s + 1];
+            len = b.kv_len[s];
+            n = begin >= 0 && end <= b.n_rows && end > begin ? end - begin : 0;
+            c = count(n, len);
+        }
         const int incl = scan_add(c);
         const int total = __builtin_amdgcn_readlane(incl, 63);
         if (item < base + total) {
-            const unsigned long long past = __ballot(base + incl > item);
-            const int at = __builtin_ctzll(past);
-            seq = __builtin_amdgcn_readfirstlane(s0 + at);
-            local = __builtin_amdgcn_readfirstlane(item - base - __builtin_amdgcn_readlane(incl - c, at));
+            const int at = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(__ballot(base + incl > item)));
+            f.seq = s0 + at;
+            f.local = item - base - __builtin_amdgcn_readlane(incl - c, at);
+            f.begin = __builtin_amdgcn_readlane(begin, at);
+            f.n = __builtin_amdgcn_readlane(n, at);
+            f.len = __builtin_amdgcn_readlane(len, at);
             return true;
         }
         base += total;

@@ -18,15 +18,10 @@ namespace {
 
 constexpr float PER127 = 0x1.020408p-7f;  // fl(1 / 127)
 
-// pages that the rows of sequence s touch, `first` their first token
-__device__ __forceinline__ int pages_touched(const DevBatch &b, int s, bool within_table, int &begin, int &n, int &first, int &len) {
-    n = seq_rows(b, s, begin);
-    len = fixed(b.kv_len + s);
-    first = len - n;
+// pages that the last n of len tokens touch; `table`: those that the page table has
+__device__ __forceinline__ int pages_touched(int n, int len, int table) {
     if (n == 0 || len <= 0) return 0;
-    int last = (len - 1) / KV_PAGE;
-    if (within_table) last = min(last, b.max_pages - 1);
-    return max(0, last - max(first, 0) / KV_PAGE + 1);
+    return max(0, min((len - 1) / KV_PAGE, table - 1) - max(len - n, 0) / KV_PAGE + 1);
 }
 
 // the largest of the wave's values, in lane 63
@@ -72,16 +67,16 @@ __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, cons
     const int tid = threadIdx.x, lane = tid & 63, g = __builtin_amdgcn_readfirstlane(tid / 64);
     const int head = blockIdx.y;
     const bool is_v = blockIdx.z;
-    int seq, local, begin, n, first, len;
-    if (!find_item(b.n_seqs, (int)blockIdx.x, [&](int s) { int x, y, z, w; return pages_touched(b, s, true, x, y, z, w); }, seq, local)) return;
-    pages_touched(b, seq, true, begin, n, first, len);
-    const int pi = max(first, 0) / KV_PAGE + local;
-    const int phys = fixed(b.pages + (int64_t)seq * b.max_pages + pi);
+    Found f;
+    if (!find_item(b, (int)blockIdx.x, [&](int n, int len) { return pages_touched(n, len, b.max_pages); }, f)) return;
+    const int len = f.len, first = len - f.n;
+    const int pi = max(first, 0) / KV_PAGE + f.local;
+    const int phys = fixed(b.pages + (int64_t)f.seq * b.max_pages + pi);
     const bool there = phys >= 0 && phys < c.n_pages;
     const int t_lo = max(first - pi * KV_PAGE, 0), t_hi = min(len - pi * KV_PAGE, KV_PAGE);  // the page's new tokens
     const T *src = is_v ? xv : xk;
     const int64_t stride = is_v ? v_stride : k_stride;
-    const int64_t row0 = (int64_t)begin + (pi * KV_PAGE - first);  // row of the page's token 0 (may lie before the sequence)
+    const int64_t row0 = (int64_t)f.begin + (pi * KV_PAGE - first);  // row of the page's token 0 (may lie before the sequence)
 
     // the values first: they are asked for before it is known which page they go to
     float x[16][VEC];
@@ -221,17 +216,17 @@ __global__ __launch_bounds__(256) void kv_read_kernel(DevKv c, DevBatch b, T *yk
     __shared__ __align__(16) uint8_t tile[KV_PAGE * PITCH];  // codes by token
     const int tid = threadIdx.x, head = blockIdx.y;
     const bool is_v = blockIdx.z;
-    int seq, local, begin, n, first, len;
-    if (!find_item(b.n_seqs, (int)blockIdx.x, [&](int s) { int x, y, z, w; return pages_touched(b, s, false, x, y, z, w); }, seq, local)) return;
-    pages_touched(b, seq, false, begin, n, first, len);
-    const int pi = max(first, 0) / KV_PAGE + local;
-    int phys = pi < b.max_pages ? fixed(b.pages + (int64_t)seq * b.max_pages + pi) : -1;
+    Found f;
+    if (!find_item(b, (int)blockIdx.x, [&](int n, int len) { return pages_touched(n, len, INT32_MAX); }, f)) return;
+    const int len = f.len, first = len - f.n;
+    const int pi = max(first, 0) / KV_PAGE + f.local;
+    int phys = pi < b.max_pages ? fixed(b.pages + (int64_t)f.seq * b.max_pages + pi) : -1;
     const bool bad = phys < 0 || phys >= c.n_pages;  // such a page's tokens read as NaN
     if (bad) phys = 0;
     const int t_lo = max(first - pi * KV_PAGE, 0), t_hi = min(len - pi * KV_PAGE, KV_PAGE);
     T *dst = is_v ? yv : yk;
     const int64_t stride = is_v ? v_stride : k_stride;
-    const int64_t row0 = (int64_t)begin + (pi * KV_PAGE - first);
+    const int64_t row0 = (int64_t)f.begin + (pi * KV_PAGE - first);
     const int64_t at = (int64_t)phys * c.kv_heads + head;
     const float *scales = (is_v ? c.vs : c.ks) + at * c.per;
     const uint8_t *codes = (is_v ? c.v : c.k) + at * (KV_PAGE * DP);
