@@ -236,22 +236,55 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
     visible(a, first + same(row0, a.group), len, lo_min, hi_min);
     visible(a, first + same(min(row0 + ROWS, rows) - 1, a.group), len, lo_max, hi_max);
 
-    // queries: dimensions 64 c + 16 g + 8 i .. + 7 of row r, as the second operand of step (c, i)
-    Halves qh[2 * NC], ql[2 * NC];
-    float score_scale, minus_bias;
+    // Everything that the rows wait for once is asked for as early as it can be: page numbers, queries, the first page.
+    int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
+    if (a.splits > 1) {
+        const int share = same(t1 - t0 + a.splits - 1, a.splits);
+        t0 = t0 + (int)blockIdx.z * share;
+        t1 = min(t1, t0 + share);
+    }
+    int ids = pages_from(a, seq, t0 + wave, 4);
+    V4 raw[NC][4];
     {
-        float x[NC][16];
-        float big = 0.f;
         const T *p = (const T *)a.q + (int64_t)(begin + my_t) * a.q_stride + (int64_t)(head * a.group + my_h) * a.c.head_dim;
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int d = 64 * c + 16 * g + 4 * i;
-                V4 y = {};
-                if (valid && d < a.c.head_dim) y = *(const V4 *)(p + d);
+                raw[c][i] = V4{};
+                if (valid && d < a.c.head_dim) raw[c][i] = *(const V4 *)(p + d);
+            }
+    }
+    uint4 kc[4][NC], vc[4 * NC];
+    float sc;
+    auto fetch = [&](int phys) {
+        const int64_t at = (int64_t)max(phys, 0) * a.c.kv_heads + head;
+        sc = scales_from(a, phys, head);
+        const uint4 *kp = (const uint4 *)(a.c.k + at * (KV_PAGE * DP)) + lane;
+        const uint4 *vp = (const uint4 *)(a.c.v + at * (KV_PAGE * DP)) + lane;
 #pragma unroll
-                for (int e = 0; e < 4; e++) { x[c][4 * i + e] = to_f32(y[e]); big = fmaxf(big, fabsf(x[c][4 * i + e])); }
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int c = 0; c < NC; c++) kc[t][c] = kp[(t * NC + c) * 64];
+#pragma unroll
+        for (int d = 0; d < 4 * NC; d++) vc[d] = vp[d * 64];
+    };
+    int phys = __builtin_amdgcn_readlane(ids, 0);
+    if (t0 + wave < t1) fetch(phys);
+
+    // queries: dimensions 64 c + 16 g + 8 i .. + 7 of row r, as the second operand of step (c, i)
+    Halves qh[2 * NC], ql[2 * NC];
+    float score_scale, minus_bias;
+    {
+        float x[NC][16];
+        float big = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                x[c][i] = to_f32(raw[c][i / 4][i % 4]);
+                big = fmaxf(big, fabsf(x[c][i]));
             }
         big = fmaxf(big, __shfl_xor(big, 16));
         big = fmaxf(big, __shfl_xor(big, 32));
@@ -285,27 +318,12 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
     float m = MINUS_INF, l = 0.f;
     float ref = 0x1p-100f, unit = 0x1p115f;  // values are accumulated in units of ref * 2^-15 = 1 / unit
 
-    int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
-    if (a.splits > 1) {
-        const int share = same(t1 - t0 + a.splits - 1, a.splits);
-        t0 = t0 + (int)blockIdx.z * share;
-        t1 = min(t1, t0 + share);
-    }
-    int ids = 0;
     for (int page = t0 + wave, k = 0; page < t1; page += 4, k++) {
-        if (k % 64 == 0) ids = pages_from(a, seq, page, 4);
-        const int phys = __builtin_amdgcn_readlane(ids, k % 64);
-        const int64_t at = (int64_t)max(phys, 0) * a.c.kv_heads + head;
-        const float sc = scales_from(a, phys, head);
-        const uint4 *kp = (const uint4 *)(a.c.k + at * (KV_PAGE * DP)) + lane;
-        const uint4 *vp = (const uint4 *)(a.c.v + at * (KV_PAGE * DP)) + lane;
-        uint4 kc[4][NC], vc[4 * NC];
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int c = 0; c < NC; c++) kc[t][c] = kp[(t * NC + c) * 64];
-#pragma unroll
-        for (int d = 0; d < 4 * NC; d++) vc[d] = vp[d * 64];
+        if (k) {
+            if (k % 64 == 0) ids = pages_from(a, seq, page, 4);
+            phys = __builtin_amdgcn_readlane(ids, k % 64);
+            fetch(phys);
+        }
         float ks[4], vs[4];
         spread_scales(sc, phys, ks, vs);
         const int j0 = page * KV_PAGE;
