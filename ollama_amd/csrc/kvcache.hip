@@ -59,6 +59,57 @@ __device__ __forceinline__ void codes_of(const float (&x)[N], float s, int (&q)[
     for (int i = 0; i < N; i++) q[i] = clamp_code(r[i]) + 128;
 }
 
+// One 16-byte piece whose bytes of `mask` hold older codes: moved to the larger scale.
+__device__ __forceinline__ void move_piece(uint8_t *p, uint32_t mask, float grown) {
+    uint32_t w[4];
+    *(uint4 *)w = *(const uint4 *)p;
+#pragma unroll
+    for (int m = 0; m < 4; m++) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int byte = (int)(w[m] >> (8 * i) & 0xff);
+            const int moved = clamp_code(rintf((float)(byte - 128) * grown)) + 128;
+            r |= (uint32_t)(mask >> (4 * m + i) & 1 ? moved : byte) << (8 * i);
+        }
+        w[m] = r;
+    }
+    *(uint4 *)p = *(const uint4 *)w;
+}
+
+// The codes of tokens lo .. hi - 1 of a page and head, moved by all threads of the workgroup; what is stored to them
+// afterwards lands on top.
+template <int VEC>
+__device__ __forceinline__ void move_codes(uint8_t *codes, bool is_v, int lo, int hi, float grown) {
+    for (int i = threadIdx.x; i < 256 * VEC; i += 256) {  // pieces in memory order
+        uint32_t mask = 0;
+        if (is_v) {
+            const int g = i % 64 / 16;
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const int t = 16 * (j / 4) + 4 * g + j % 4;
+                mask |= (uint32_t)(t >= lo && t < hi) << j;
+            }
+        } else {
+            const int t = i / (64 * VEC) * 16 + i % 16;
+            mask = t >= lo && t < hi ? 0xffffu : 0u;
+        }
+        if (mask) move_piece(codes + (int64_t)i * 16, mask, grown);
+    }
+    __syncthreads();
+}
+
+// the block's scale: its older tokens' if there are any and it holds the new largest magnitude (a bit pattern: ordered
+// like the numbers, infinity and NaN above all); grown: old / new where the older codes have to move
+__device__ __forceinline__ float block_scale(uint32_t big, bool going_on, float old, float &grown, bool &moves) {
+    float s = big >= 0x7f800000u ? __builtin_nanf("") : __uint_as_float(big) * PER127;
+    if (going_on) {
+        if (s <= old || old != old) s = old;
+        else if (s > old) { grown = old / s; moves = true; }
+    }
+    return s;
+}
+
 template <class T, int VEC>
 __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, const T *xk, const T *xv, int64_t k_stride, int64_t v_stride) {
     constexpr int DP = 64 * VEC, PITCH = DP + 16;
@@ -77,10 +128,63 @@ __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, cons
     const T *src = is_v ? xv : xk;
     const int64_t stride = is_v ? v_stride : k_stride;
     const int64_t row0 = (int64_t)f.begin + (pi * KV_PAGE - first);  // row of the page's token 0 (may lie before the sequence)
+    const bool live = lane * VEC < c.head_dim;
+    const int64_t at = (int64_t)(there ? phys : 0) * c.kv_heads + head;
+    float *scales = (is_v ? c.vs : c.ks) + at * c.per;
+    uint8_t *codes = (is_v ? c.v : c.k) + at * (KV_PAGE * DP);
+    const int going_on = t_lo % c.block ? t_lo / c.block : -1;  // the block that holds older tokens
+    float grown = 0.f;
+    bool moves = false;
+
+    // A step of few tokens: a wave each, its codes stored byte by byte.  The page's way below would be 20 KiB of code to
+    // fetch for one token.
+    if (t_hi - t_lo <= 4) {
+        const int t = t_lo + g;
+        float x[VEC];
+        uint32_t big = 0;
+#pragma unroll
+        for (int v = 0; v < VEC; v++) x[v] = 0.f;
+        if (t < t_hi) {
+            const T *p = src + (row0 + t) * stride + (int64_t)head * c.head_dim + lane * VEC;
+#pragma unroll
+            for (int v = 0; v < VEC; v++) {
+                if (live && lane * VEC + v < c.head_dim) x[v] = to_f32(p[v]);
+                big = max(big, __float_as_uint(x[v]) & 0x7fffffffu);
+            }
+        }
+        if (!there) return;
+        const float old = going_on >= 0 ? scales[going_on] : 0.f;
+        big = wave_umax(big);
+        if (lane == 63) largest[0][g] = big;
+        __syncthreads();
+        const int block0 = t_lo / c.block, mine = min(t, t_hi - 1) / c.block;  // few tokens lie in two blocks at most
+        uint32_t mx0 = 0, mx1 = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (t_lo + i >= t_hi) continue;
+            if ((t_lo + i) / c.block == block0) mx0 = max(mx0, largest[0][i]);
+            else mx1 = max(mx1, largest[0][i]);
+        }
+        const float s0 = block_scale(mx0, going_on >= 0, old, grown, moves), s1 = block_scale(mx1, false, 0.f, grown, moves);
+        if (moves) move_codes<VEC>(codes, is_v, going_on * c.block, t_lo, grown);
+        if (t >= t_hi) return;
+        const float s = mine == block0 ? s0 : s1;
+        if (lane == 0) scales[mine] = s;  // the tokens of a block write the same
+        int q[VEC];
+        codes_of(x, s, q);
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+            const int d = lane * VEC + v;
+            if (d >= c.head_dim) continue;
+            const int place = is_v ? ((d / 16 * 4 + t % 16 / 4) * 16 + d % 16) * 16 + t / 16 * 4 + t % 4
+                                   : (((t / 16 * VEC + d / 64) * 4 + d % 64 / 16) * 16 + t % 16) * 16 + d % 16;
+            codes[place] = (uint8_t)q[v];
+        }
+        return;
+    }
 
     // the values first: they are asked for before it is known which page they go to
     float x[16][VEC];
-    const bool live = lane * VEC < c.head_dim;
 #pragma unroll
     for (int j = 0; j < 16; j++) {
         const int t = 16 * (j / 4) + 4 * g + j % 4;
@@ -94,14 +198,10 @@ __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, cons
         }
     }
     if (!there) return;
-    const int64_t at = (int64_t)phys * c.kv_heads + head;
-    float *scales = (is_v ? c.vs : c.ks) + at * c.per;
-    uint8_t *codes = (is_v ? c.v : c.k) + at * (KV_PAGE * DP);
-    const int going_on = t_lo % c.block ? t_lo / c.block : -1;  // the block that holds older tokens
     const float old = going_on >= 0 ? scales[going_on] : 0.f;
 #pragma unroll
     for (int m = 0; m < 4; m++) {
-        uint32_t big = 0;  // magnitudes as bit patterns: ordered like the numbers, infinity and NaN above all
+        uint32_t big = 0;
 #pragma unroll
         for (int j = 4 * m; j < 4 * m + 4; j++)
 #pragma unroll
@@ -110,8 +210,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, cons
         if (lane == 63) largest[g][m] = big;
     }
     __syncthreads();
-    float s[4], grown = 0.f;  // scale of the block that 16 tokens belong to; old scale / new scale where older codes move
-    bool moves = false;
+    float s[4];  // scale of the block that 16 tokens belong to
     {
         uint32_t mx[4];
 #pragma unroll
@@ -119,52 +218,33 @@ __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, cons
         if (c.block >= 32) { mx[0] = mx[1] = max(mx[0], mx[1]); mx[2] = mx[3] = max(mx[2], mx[3]); }
         if (c.block >= 64) { mx[0] = mx[1] = mx[2] = mx[3] = max(mx[0], mx[2]); }
 #pragma unroll
-        for (int m = 0; m < 4; m++) {
-            s[m] = mx[m] >= 0x7f800000u ? __builtin_nanf("") : __uint_as_float(mx[m]) * PER127;
-            if (16 * m / c.block == going_on) {
-                if (s[m] <= old || old != old) s[m] = old;
-                else if (s[m] > old) { grown = old / s[m]; moves = true; }
-            }
-        }
+        for (int m = 0; m < 4; m++) s[m] = block_scale(mx[m], 16 * m / c.block == going_on, old, grown, moves);
     }
-    const int moved_lo = moves ? going_on * c.block : t_lo;  // tokens moved_lo .. t_lo - 1 get new codes too
+    if (moves) move_codes<VEC>(codes, is_v, going_on * c.block, t_lo, grown);
     if (tid < c.per && tid >= t_lo / c.block && tid <= (t_hi - 1) / c.block) {
         const int m = tid * c.block / 16;
         scales[tid] = m < 2 ? (m == 0 ? s[0] : s[1]) : (m == 2 ? s[2] : s[3]);
     }
-
     int q[16][VEC];
 #pragma unroll
     for (int j = 0; j < 16; j++) {
         const int t = 16 * (j / 4) + 4 * g + j % 4;
         if (t >= t_lo && t < t_hi) codes_of(x[j], s[j / 4], q[j]);
     }
-
     if (is_v) {
-        bool any = false, all = true;
+        bool all = true;
 #pragma unroll
         for (int j = 0; j < 16; j++) {
             const int t = 16 * (j / 4) + 4 * g + j % 4;
-            any |= t >= moved_lo && t < t_hi;
             all &= t >= t_lo && t < t_hi;
         }
-        if (!any) return;
 #pragma unroll
         for (int v = 0; v < VEC; v++) {
             const int d = lane * VEC + v;
             if (d >= c.head_dim) continue;
             uint8_t *piece = codes + (((d / 16) * 4 + g) * 16 + d % 16) * 16;
-            uint32_t w[4];
-            if (moves) {
-                *(uint4 *)w = *(const uint4 *)piece;
-#pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const int t = 16 * (j / 4) + 4 * g + j % 4;
-                    const int byte = (int)(w[j / 4] >> (8 * (j % 4)) & 0xff) - 128;
-                    if (t >= moved_lo && t < t_lo) piece[j] = (uint8_t)(clamp_code(rintf((float)byte * grown)) + 128);
-                }
-            }
             if (all) {
+                uint32_t w[4];
 #pragma unroll
                 for (int m = 0; m < 4; m++)
                     w[m] = (uint32_t)q[4 * m][v] | (uint32_t)q[4 * m + 1][v] << 8 | (uint32_t)q[4 * m + 2][v] << 16 | (uint32_t)q[4 * m + 3][v] << 24;
@@ -191,21 +271,8 @@ __global__ __launch_bounds__(256) void kv_write_kernel(DevKv c, DevBatch b, cons
 #pragma unroll
     for (int e = 0; e < VEC; e++) {  // pieces (64 dimensions e, 16 of them, token), token fastest
         const int t = tid & 63, p = tid / 64;
-        uint4 *piece = (uint4 *)(codes + (((t / 16 * VEC + e) * 4 + p) * 16 + t % 16) * 16);
-        if (t >= t_lo && t < t_hi) {
-            *piece = *(const uint4 *)(tile + t * PITCH + e * 64 + p * 16);
-        } else if (t >= moved_lo && t < t_lo) {
-            uint32_t w[4];
-            *(uint4 *)w = *piece;
-#pragma unroll
-            for (int m = 0; m < 4; m++) {
-                uint32_t r = 0;
-#pragma unroll
-                for (int i = 0; i < 4; i++) r |= (uint32_t)(clamp_code(rintf((float)((int)(w[m] >> (8 * i) & 0xff) - 128) * grown)) + 128) << (8 * i);
-                w[m] = r;
-            }
-            *piece = *(uint4 *)w;
-        }
+        if (t >= t_lo && t < t_hi)
+            *(uint4 *)(codes + (((t / 16 * VEC + e) * 4 + p) * 16 + t % 16) * 16) = *(const uint4 *)(tile + t * PITCH + e * 64 + p * 16);
     }
 }
 
