@@ -34,6 +34,14 @@ typedef float float16v __attribute__((ext_vector_type(16)));
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float MINUS_INF = -__builtin_inff();
 
+// one of the two ways that rows are worked on: tiles of 16 or of 128 rows
+struct Share {
+    float *part;      // [item][kv head][split]: R x dp numerators, R maxima, R sums (R rows per tile)
+    int items;        // tiles at most; 0: none
+    int splits;       // workgroups that a tile's cache is cut over
+    int least, most;  // sequences of least..most (token, head) rows per key/value head
+};
+
 struct AttnLaunch {
     DevKv c;
     DevBatch b;
@@ -44,10 +52,8 @@ struct AttnLaunch {
     float scale, softcap;
     int causal, window;
     const float *sinks;
-    float *part;  // [item][kv head][split]: R x dp numerators, R maxima, R sums (R rows per tile)
-    int splits, items;
-    int shift;        // groups of 16 tokens per scale, as a power of two
-    int most, least;  // sequences of least..most (token, head) rows per key/value head are this launch's
+    int shift;  // groups of 16 tokens per scale, as a power of two
+    Share few, many;
 };
 
 union Halves {
@@ -89,11 +95,11 @@ __device__ __forceinline__ float settled(float x) {
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
 __device__ __forceinline__ int exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 0xff) - 127; }
 
-// tiles of R rows that this launch has in a sequence of n rows
+// tiles of R rows that a share has in a sequence of n rows
 template <int R>
-__device__ __forceinline__ int tiles_of(const AttnLaunch &a, int n) {
-    const int rows = n * a.group;
-    return rows >= a.least && rows <= a.most ? (rows + R - 1) / R : 0;
+__device__ __forceinline__ int tiles_of(const Share &s, int group, int n) {
+    const int rows = n * group;
+    return rows >= s.least && rows <= s.most ? (rows + R - 1) / R : 0;
 }
 
 // the value of the lane 32 away, exchanged in the registers
@@ -212,19 +218,24 @@ __device__ __forceinline__ void take_out_nan(float (&ks)[4], float (&vs)[4], int
 // cache is split over workgroups a second kernel joins those.
 constexpr int ROWS = 16;
 
+struct RowsLds {
+    float o[4][ROWS][64 + 4];
+    float m[4][ROWS], l[4][ROWS];
+};
+
+// work: the workgroup's number among the share's, heads fastest
 template <class T, int NC, bool CAP>
-__global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
+__device__ __forceinline__ void attn_rows(const AttnLaunch &a, RowsLds &lds, int work) {
     constexpr bool HILO = sizeof(T) == 4;                // queries in two halves
     constexpr bool PHILO = !__is_same(T, __bf16);  // probabilities in two halves
     constexpr int DP = 64 * NC;
     using V4 = typename Vec4<T>::type;
-    __shared__ float part_o[4][ROWS][64 + 4];
-    __shared__ float part_m[4][ROWS], part_l[4][ROWS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const int r = lane % 16, g = lane / 16;
-    const int head = blockIdx.y;  // key/value head
+    const int rest = same(work, a.c.kv_heads), head = work - rest * a.c.kv_heads;  // key/value head
+    const int split = same(rest, a.few.items), item = rest - split * a.few.items;
     Found at_item;
-    if (!find_item(a.b, (int)blockIdx.x, [&](int n, int) { return tiles_of<ROWS>(a, n); }, at_item)) return;
+    if (!find_item(a.b, item, [&](int n, int) { return tiles_of<ROWS>(a.few, a.group, n); }, at_item)) return;
     const int seq = at_item.seq, tile = at_item.local, begin = at_item.begin;
     const int n = at_item.n, len = at_item.len, first = len - n;
     const int rows = n * a.group, row0 = tile * ROWS;
@@ -238,9 +249,9 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
 
     // Everything that the rows wait for once is asked for as early as it can be: page numbers, queries, the first page.
     int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
-    if (a.splits > 1) {
-        const int share = same(t1 - t0 + a.splits - 1, a.splits);
-        t0 = t0 + (int)blockIdx.z * share;
+    if (a.few.splits > 1) {
+        const int share = same(t1 - t0 + a.few.splits - 1, a.few.splits);
+        t0 = t0 + split * share;
         t1 = min(t1, t0 + share);
     }
     int ids = pages_from(a, seq, t0 + wave, 4);
@@ -403,14 +414,14 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
     // the four waves' results joined: 64 dimensions at a time through LDS
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (g == 0) { part_m[wave][r] = m; part_l[wave][r] = l; }
+    if (g == 0) { lds.m[wave][r] = m; lds.l[wave][r] = l; }
     __syncthreads();
     auto joined = [&](int row, float &top, float &base, float &sum) {
-        top = fmaxf(fmaxf(part_m[0][row], part_m[1][row]), fmaxf(part_m[2][row], part_m[3][row]));
+        top = fmaxf(fmaxf(lds.m[0][row], lds.m[1][row]), fmaxf(lds.m[2][row], lds.m[3][row]));
         base = top == MINUS_INF ? 0.f : top;
         sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) sum += __builtin_amdgcn_exp2f(part_m[w][row] - base) * part_l[w][row];
+        for (int w = 0; w < 4; w++) sum += __builtin_amdgcn_exp2f(lds.m[w][row] - base) * lds.l[w][row];
     };
     float top, base, sum;
     joined(r, top, base, sum);
@@ -420,10 +431,10 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
     const bool writes = row0 + o_row < rows;
     const int o_t = writes ? (row0 + o_row) / a.group : 0, o_h = head * a.group + (writes ? row0 + o_row - o_t * a.group : 0);
     joined(o_row, top, base, sum);
-    const int64_t index = ((int64_t)blockIdx.x * a.c.kv_heads + head) * a.splits + blockIdx.z;
-    float *part = a.part + index * (ROWS * (DP + 2));
+    const int64_t index = ((int64_t)item * a.c.kv_heads + head) * a.few.splits + split;
+    float *part = a.few.part + index * (ROWS * (DP + 2));
     float divide = 1.f;
-    if (a.splits == 1) {
+    if (a.few.splits == 1) {
         float total = sum;
         if (a.sinks) {
             const float sink = a.sinks[o_h] * LOG2E, all = fmaxf(base, sink);
@@ -445,19 +456,19 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
             float4v y = acc[4 * c + d];
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] *= weight;
-            *(float4v *)&part_o[wave][r][16 * d + 4 * g] = y;
+            *(float4v *)&lds.o[wave][r][16 * d + 4 * g] = y;
         }
         __syncthreads();
-        float4v y = *(const float4v *)&part_o[0][o_row][o_d];
+        float4v y = *(const float4v *)&lds.o[0][o_row][o_d];
 #pragma unroll
         for (int w = 1; w < 4; w++) {
-            const float4v x = *(const float4v *)&part_o[w][o_row][o_d];
+            const float4v x = *(const float4v *)&lds.o[w][o_row][o_d];
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] += x[e];
         }
         const int d = 64 * c + o_d;
         if (!writes || d >= a.c.head_dim) continue;
-        if (a.splits == 1) {
+        if (a.few.splits == 1) {
             V4 w;
 #pragma unroll
             for (int e = 0; e < 4; e++) w[e] = (T)(sum == 0.f ? 0.f : y[e] * divide);
@@ -466,6 +477,12 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
             *(float4v *)(part + o_row * DP + d) = y;
         }
     }
+}
+
+template <class T, int NC, bool CAP>
+__global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
+    __shared__ RowsLds lds;
+    attn_rows<T, NC, CAP>(a, lds, (int)blockIdx.x);
 }
 
 // ---- 128 rows per workgroup: prompts ----------------------------------------------------------------------------------
@@ -477,18 +494,18 @@ constexpr int TILE = 128;
 constexpr float LAZY = 6.f;
 
 template <class T, int NC, bool CAP>
-__global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLaunch a) {
+__device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int work) {
     constexpr bool HILO = sizeof(T) == 4;              // queries in two halves
     constexpr bool PHILO = !__is_same(T, __bf16);      // probabilities in two halves
     constexpr int DP = 64 * NC, BYTES = KV_PAGE * DP;  // of a page's keys (and values) of one head
     using V4 = typename Vec4<T>::type;
-    extern __shared__ __align__(1024) uint8_t lds[];  // two buffers of a page's keys and values as halves
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const int r = lane % 32, h = lane / 32;
     // heads fastest: with eight of them every XCD keeps one head's cache in its L2; later tiles (longer ones) first
-    const int head = blockIdx.x % a.c.kv_heads, item = a.items - 1 - (int)blockIdx.x / a.c.kv_heads;
+    const int rest = same(work, a.c.kv_heads), head = work - rest * a.c.kv_heads;
+    const int nth = same(rest, a.many.splits), split = rest - nth * a.many.splits, item = a.many.items - 1 - nth;
     Found at_item;
-    if (!find_item(a.b, item, [&](int n, int) { return tiles_of<TILE>(a, n); }, at_item)) return;
+    if (!find_item(a.b, item, [&](int n, int) { return tiles_of<TILE>(a.many, a.group, n); }, at_item)) return;
     const int seq = at_item.seq, tile = at_item.local, begin = at_item.begin;
     const int n = at_item.n, len = at_item.len, first = len - n;
     const int rows = n * a.group, row0 = tile * TILE, wrow0 = row0 + 32 * wave;
@@ -503,9 +520,9 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
 
     // Everything that a tile waits for once is asked for as early as it can be: page numbers, queries, the first page.
     int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
-    if (a.splits > 1) {
-        const int share = same(t1 - t0 + a.splits - 1, a.splits);
-        t0 = t0 + (int)blockIdx.z * share;
+    if (a.many.splits > 1) {
+        const int share = same(t1 - t0 + a.many.splits - 1, a.many.splits);
+        t0 = t0 + split * share;
         t1 = min(t1, t0 + share);
     }
     int ids = pages_from(a, seq, t0, 1);  // this page's, the next one's and the one after's number; scales of the first two
@@ -755,9 +772,9 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
     const int o_h = head * a.group + my_h;
     const float base = m == MINUS_INF ? 0.f : m;
     float weight = ref * 0x1p-9f;
-    float *part = a.part + (((int64_t)item * a.c.kv_heads + head) * a.splits + blockIdx.z) * (TILE * (DP + 2));
+    float *part = a.many.part + (((int64_t)item * a.c.kv_heads + head) * a.many.splits + split) * (TILE * (DP + 2));
     const int in_tile = 32 * wave + r;
-    if (a.splits == 1) {
+    if (a.many.splits == 1) {
         float total = l, scale = 1.f;
         if (a.sinks) {
             const float sink = a.sinks[o_h] * LOG2E, all = fmaxf(base, sink);
@@ -779,7 +796,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
             float4v y;
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] = l == 0.f ? 0.f : acc[d][4 * i + e] * weight;
-            if (a.splits == 1) {
+            if (a.many.splits == 1) {
                 V4 z;
 #pragma unroll
                 for (int e = 0; e < 4; e++) z[e] = (T)y[e];
@@ -790,31 +807,42 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
         }
 }
 
+// Prompts, and in the same launch the sequences of few rows beside them: those first, so that single tokens are done while
+// the prompts are worked on.
+template <class T, int NC, bool CAP>
+__global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLaunch a) {
+    extern __shared__ __align__(1024) uint8_t lds[];  // two buffers of a page's keys and values as halves
+    const int few = a.few.items * a.few.splits * a.c.kv_heads;
+    if ((int)blockIdx.x < few) attn_rows<T, NC, CAP>(a, *(RowsLds *)lds, (int)blockIdx.x);
+    else attn_tile<T, NC, CAP>(a, lds, (int)blockIdx.x - few);
+}
+
 // The splits of a tile joined.  Bound by the latency of its three dependent rounds of loads (which sequence, the partial
 // results, the sinks): a thread takes four dimensions of one row and asks for eight splits' numerators and sums at a time,
 // before it knows their maximum.
 template <class T, int R>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnLaunch a) {
+    const Share &share = R == ROWS ? a.few : a.many;
     using V4 = typename Vec4<T>::type;
     const int head = blockIdx.y, dp = a.c.dp, quads = a.c.head_dim / 4;
     Found at_item;
-    if (!find_item(a.b, (int)blockIdx.x, [&](int n, int) { return tiles_of<R>(a, n); }, at_item)) return;
+    if (!find_item(a.b, (int)blockIdx.x, [&](int n, int) { return tiles_of<R>(share, a.group, n); }, at_item)) return;
     const int tile = at_item.local, begin = at_item.begin, n = at_item.n;
     const int rows = min(R, n * a.group - tile * R);
     const int64_t size = R * (dp + 2);
-    const float *part = a.part + ((int64_t)blockIdx.x * a.c.kv_heads + head) * a.splits * size;
+    const float *part = share.part + ((int64_t)blockIdx.x * a.c.kv_heads + head) * share.splits * size;
     for (int i = threadIdx.x + blockIdx.z * 256; i < rows * quads; i += 256 * gridDim.z) {
         const int row = i / quads, d = (i - row * quads) * 4;
         const int t = (tile * R + row) / a.group, h = head * a.group + tile * R + row - t * a.group;
         float top = MINUS_INF, sum = 0.f;
         float4v y = {0.f, 0.f, 0.f, 0.f};
         const float sink = a.sinks ? a.sinks[h] * LOG2E : MINUS_INF;
-        for (int s0 = 0; s0 < a.splits; s0 += 8) {
+        for (int s0 = 0; s0 < share.splits; s0 += 8) {
             float m[8], l[8];
             float4v x[8];
 #pragma unroll
             for (int s = 0; s < 8; s++) {
-                const float *p = part + min(s0 + s, a.splits - 1) * size;
+                const float *p = part + min(s0 + s, share.splits - 1) * size;
                 m[s] = p[R * dp + row];
                 l[s] = p[R * dp + R + row];
                 x[s] = *(const float4v *)(p + row * dp + d);
@@ -829,7 +857,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnLaunch a) {
             for (int e = 0; e < 4; e++) y[e] *= keep;
 #pragma unroll
             for (int s = 0; s < 8; s++) {
-                if (s0 + s >= a.splits || l[s] == 0.f) continue;  // a split that saw nothing has no numerators
+                if (s0 + s >= share.splits || l[s] == 0.f) continue;  // a split that saw nothing has no numerators
                 const float w = __builtin_amdgcn_exp2f(m[s] - base);
                 sum += l[s] * w;
 #pragma unroll
@@ -846,54 +874,47 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnLaunch a) {
     }
 }
 
-template <class T, int NC, int R>
+template <class T, int NC>
 hipError_t launch_one(const AttnLaunch &a, hipStream_t s) {
-    if (R == ROWS) {
-        const dim3 grid((unsigned)a.items, (unsigned)a.c.kv_heads, (unsigned)a.splits);
-        if (a.softcap > 0.f) attn_rows_kernel<T, NC, true><<<grid, 256, 0, s>>>(a);
-        else attn_rows_kernel<T, NC, false><<<grid, 256, 0, s>>>(a);
+    const unsigned few = (unsigned)a.few.items * (unsigned)a.few.splits * (unsigned)a.c.kv_heads;
+    const unsigned many = (unsigned)a.many.items * (unsigned)a.many.splits * (unsigned)a.c.kv_heads;
+    if (!many) {
+        if (a.softcap > 0.f) attn_rows_kernel<T, NC, true><<<few, 256, 0, s>>>(a);
+        else attn_rows_kernel<T, NC, false><<<few, 256, 0, s>>>(a);
     } else {
-        const dim3 grid((unsigned)a.items * (unsigned)a.c.kv_heads, 1, (unsigned)a.splits);
         const auto kernel = a.softcap > 0.f ? attn_tile_kernel<T, NC, true> : attn_tile_kernel<T, NC, false>;
         constexpr int lds = 2 * 4 * KV_PAGE * 64 * NC;
+        static_assert(lds >= (int)sizeof(RowsLds), "the 16-row way shares the buffers");
         if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        kernel<<<grid, 256, lds, s>>>(a);
+        kernel<<<few + many, 256, lds, s>>>(a);
     }
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.splits == 1) return e;
-    // 256 threads take 8 rows of 128; a tile of 128 rows is given to 16 workgroups
-    attn_join_kernel<T, R><<<dim3((unsigned)a.items, (unsigned)a.c.kv_heads, R == ROWS ? 1 : 16), 256, 0, s>>>(a);
-    return hipGetLastError();
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && few && a.few.splits > 1) {
+        attn_join_kernel<T, ROWS><<<dim3((unsigned)a.few.items, (unsigned)a.c.kv_heads), 256, 0, s>>>(a);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess && many && a.many.splits > 1) {  // 256 threads take 8 rows of 128: a tile is given to 16 workgroups
+        attn_join_kernel<T, TILE><<<dim3((unsigned)a.many.items, (unsigned)a.c.kv_heads, 16), 256, 0, s>>>(a);
+        e = hipGetLastError();
+    }
+    return e;
 }
 
-template <class T, int R>
+template <class T>
 hipError_t launch_t(const AttnLaunch &a, hipStream_t s) {
     switch (a.c.dp / 64) {
-    case 1: return launch_one<T, 1, R>(a, s);
-    case 2: return launch_one<T, 2, R>(a, s);
-    case 3: return launch_one<T, 3, R>(a, s);
-    default: return launch_one<T, 4, R>(a, s);
+    case 1: return launch_one<T, 1>(a, s);
+    case 2: return launch_one<T, 2>(a, s);
+    case 3: return launch_one<T, 3>(a, s);
+    default: return launch_one<T, 4>(a, s);
     }
 }
 
-template <int R>
-hipError_t launch_type(const AttnLaunch &a, int type, hipStream_t s) {
-    if (type == T_F32) return launch_t<float, R>(a, s);
-    if (type == T_F16) return launch_t<_Float16, R>(a, s);
-    return launch_t<__bf16, R>(a, s);
-}
-
-// Sequences of at most FEW (token, head) rows per key/value head go to the 16-row kernel, longer ones to the 128-row one.
+// Sequences of at most FEW (token, head) rows per key/value head go the 16-row way, longer ones the 128-row way.
 constexpr int FEW = 32;
 
-struct Plan {
-    int64_t items;  // tiles at most; 0: no launch
-    int splits, least, most;
-    size_t floats;  // of partial results
-};
-
-// Splits of the cache for `work` workgroups without, `slots` of which run at a time.  Tiles that fill the device are not
-// split (a split tile's partial results are written and read once more, at 128 rows a third of the kernel's own time on
+// Workgroups that share a tile's cache, for `work` without and `slots` that run at a time.  Tiles that fill the device are
+// not split (a split tile's partial results are written and read once more, at 128 rows a third of the kernel's own time on
 // prompts of 4096); fewer are, so that they fill it, while a split keeps four pages.
 int splits_for(int64_t work, int64_t slots, int64_t pages) {
     int64_t s = slots / work;
@@ -901,68 +922,67 @@ int splits_for(int64_t work, int64_t slots, int64_t pages) {
     return s < 1 ? 1 : s > 32 ? 32 : (int)s;
 }
 
-void plans_of(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus, Plan &few, Plan &many) {
+// Both shares with their splits; part is left to the caller.  floats: the partial results of each.
+void shares_of(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus, Share &few, Share &many, size_t floats[2]) {
     const int64_t group = d.n_heads / c.kv_heads, all = b.n_rows * group;
     const int64_t active = b.n_seqs < b.n_rows ? b.n_seqs : b.n_rows;
-    few = many = Plan{0, 1, 1, INT32_MAX, 0};
-    // a row per sequence or few in all: the 16-row kernel; one sequence: either; otherwise both kernels look for theirs
+    few = many = Share{nullptr, 0, 1, 1, INT32_MAX};
+    floats[0] = floats[1] = 0;
+    // what a tile of `rows` rows may see: they are at most that many tokens one after the other
+    auto pages_seen = [&](int64_t rows) {
+        const int64_t w = d.window > 0 && d.causal ? (d.window + rows) / KV_PAGE + 2 : b.max_pages;
+        return w < b.max_pages ? w : (int64_t)b.max_pages;
+    };
+    // a row per sequence, or few in all: the 16-row way; one sequence: either; otherwise a launch looks for both
     const bool some_many = all > FEW && b.n_rows > b.n_seqs, some_few = b.n_seqs > 1 || !some_many;
     if (some_few) {
-        few.items = (all + (ROWS - 1) * active) / ROWS;
+        int64_t items = (all + (ROWS - 1) * active) / ROWS, most = (pages_seen(ROWS) + 3) / 4, want;
         if (some_many) {
             few.most = FEW;
             const int64_t cap = active * ((FEW + ROWS - 1) / ROWS);
-            if (few.items > cap) few.items = cap;
+            if (items > cap) items = cap;
+            // beside prompts: 64 pages per workgroup (16 rounds of its four waves, about 20 us) are done before a prompt is,
+            // and up to that length no second launch has to join anything
+            want = (pages_seen(ROWS) + 63) / 64;
+        } else {
+            // about eight workgroups per CU (rounds of them even out sequences of different lengths), down to a page per wave
+            want = 8ll * num_cus / (items * c.kv_heads) + 1;
         }
-        int64_t pages = b.max_pages;
-        if (d.window > 0 && d.causal) {  // a tile's rows are at most 16 tokens one after the other
-            const int64_t w = ((int64_t)d.window + ROWS) / KV_PAGE + 2;
-            if (w < pages) pages = w;
-        }
-        // about eight workgroups per CU (rounds of them even out sequences of different lengths), down to a page per wave
-        const int64_t want = 8ll * num_cus / (few.items * c.kv_heads) + 1, most = (pages + 3) / 4;
+        few.items = (int)items;
         few.splits = (int)(want < most ? want : most);
         if (few.splits < 1) few.splits = 1;
         if (few.splits > 256) few.splits = 256;
-        if (few.splits > 1) few.floats = (size_t)few.items * c.kv_heads * few.splits * (ROWS * (size_t)(c.dp + 2));
+        if (few.splits > 1) floats[0] = (size_t)items * c.kv_heads * few.splits * (ROWS * (size_t)(c.dp + 2));
     }
     if (some_many) {
         const int64_t seqs = all / (FEW + 1) < active ? all / (FEW + 1) : active;  // sequences that can be longer than FEW
-        many.items = (all + (TILE - 1) * seqs) / TILE;
+        many.items = (int)((all + (TILE - 1) * seqs) / TILE);
         if (b.n_seqs > 1) many.least = FEW + 1;
-        int64_t pages = b.max_pages;
-        if (d.window > 0 && d.causal) {
-            const int64_t w = ((int64_t)d.window + TILE) / KV_PAGE + 2;
-            if (w < pages) pages = w;
-        }
-        many.splits = splits_for(many.items * c.kv_heads, (c.dp <= 128 ? 2 : 1) * num_cus, pages);
-        if (many.splits > 1) many.floats = (size_t)many.items * c.kv_heads * many.splits * (TILE * (size_t)(c.dp + 2));
+        many.splits = splits_for((int64_t)many.items * c.kv_heads, (c.dp <= 128 ? 2 : 1) * num_cus, pages_seen(TILE));
+        if (many.splits > 1) floats[1] = (size_t)many.items * c.kv_heads * many.splits * (TILE * (size_t)(c.dp + 2));
     }
 }
 
 }  // namespace
 
 size_t attn_workspace_floats(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus) {
-    Plan few, many;
-    plans_of(c, b, d, num_cus, few, many);
-    return few.floats + many.floats;
+    Share few, many;
+    size_t floats[2];
+    shares_of(c, b, d, num_cus, few, many, floats);
+    return floats[0] + floats[1];
 }
 
 hipError_t launch_attention(const DevKv &c, const DevBatch &b, const AttnDesc &d, const void *q, int64_t q_stride, void *out,
                             int64_t out_stride, float *workspace, int num_cus, hipStream_t s) {
-    Plan few, many;
-    plans_of(c, b, d, num_cus, few, many);
     AttnLaunch a{c, b, q, out, q_stride, out_stride, d.n_heads, d.n_heads / c.kv_heads, d.scale, d.softcap, d.causal, d.window,
-                 d.sinks, nullptr, 1, 0, c.block == 16 ? 0 : c.block == 32 ? 1 : 2, 0, 0};
-    for (int i = 0; i < 2; i++) {
-        const Plan &p = i ? few : many;
-        if (!p.items) continue;
-        a.part = workspace + (i ? many.floats : 0);
-        a.splits = p.splits; a.items = (int)p.items; a.most = p.most; a.least = p.least;
-        const hipError_t e = i ? launch_type<ROWS>(a, d.type, s) : launch_type<TILE>(a, d.type, s);
-        if (e != hipSuccess) return e;
-    }
-    return hipSuccess;
+                 d.sinks, c.block == 16 ? 0 : c.block == 32 ? 1 : 2, Share{}, Share{}};
+    size_t floats[2];
+    shares_of(c, b, d, num_cus, a.few, a.many, floats);
+    a.few.part = workspace;
+    a.many.part = workspace + floats[0];
+    if (d.type == T_F32) return launch_t<float>(a, s);
+    if (d.type == T_F16) return launch_t<_Float16>(a, s);
+    return launch_t<__bf16>(a, s);
 }
 
 }  // namespace miqmm
