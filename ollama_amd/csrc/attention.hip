@@ -54,6 +54,7 @@ struct AttnLaunch {
     const float *sinks;
     int shift;  // groups of 16 tokens per scale, as a power of two
     Share few, many;
+    Divisor by_group, by_heads, by_few_items, by_few_splits, by_many_splits, by_quads;
 };
 
 union Halves {
@@ -137,9 +138,6 @@ __device__ __forceinline__ void cap_scores(float (&x)[N], float c) {
         for (int i = 0; i < N; i++) x[i] = c * tanhf(x[i]);
     }
 }
-
-// a / b where both are the same for the whole wave (a division is vector code: its result goes back to a scalar register)
-__device__ __forceinline__ int same(int a, int b) { return __builtin_amdgcn_readfirstlane(a / b); }
 
 // Numbers of a sequence's pages, 64 at a time in the lanes of a register: pages from + step * (0 .. 63).  Neither they nor
 // the scales go through scalar loads: those share their counter with LDS reads and come back in any order, so every LDS
@@ -232,25 +230,25 @@ __device__ __forceinline__ void attn_rows(const AttnLaunch &a, RowsLds &lds, int
     using V4 = typename Vec4<T>::type;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const int r = lane % 16, g = lane / 16;
-    const int rest = same(work, a.c.kv_heads), head = work - rest * a.c.kv_heads;  // key/value head
-    const int split = same(rest, a.few.items), item = rest - split * a.few.items;
+    const int rest = divided(work, a.by_heads), head = work - rest * a.c.kv_heads;  // key/value head
+    const int split = divided(rest, a.by_few_items), item = rest - split * a.few.items;
     Found at_item;
     if (!find_item(a.b, item, [&](int n, int) { return tiles_of<ROWS>(a.few, a.group, n); }, at_item)) return;
     const int seq = at_item.seq, tile = at_item.local, begin = at_item.begin;
     const int n = at_item.n, len = at_item.len, first = len - n;
     const int rows = n * a.group, row0 = tile * ROWS;
     const bool valid = row0 + r < rows;
-    const int my_t = valid ? (row0 + r) / a.group : 0, my_h = valid ? row0 + r - my_t * a.group : 0;
+    const int my_t = valid ? divided(row0 + r, a.by_group) : 0, my_h = valid ? row0 + r - my_t * a.group : 0;
     int lo, hi;
     visible(a, first + my_t, len, lo, hi);
     int lo_min, lo_max, hi_min, hi_max;  // over the tile's rows: both bounds grow with the row
-    visible(a, first + same(row0, a.group), len, lo_min, hi_min);
-    visible(a, first + same(min(row0 + ROWS, rows) - 1, a.group), len, lo_max, hi_max);
+    visible(a, first + divided(row0, a.by_group), len, lo_min, hi_min);
+    visible(a, first + divided(min(row0 + ROWS, rows) - 1, a.by_group), len, lo_max, hi_max);
 
     // Everything that the rows wait for once is asked for as early as it can be: page numbers, queries, the first page.
     int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
     if (a.few.splits > 1) {
-        const int share = same(t1 - t0 + a.few.splits - 1, a.few.splits);
+        const int share = divided(t1 - t0 + a.few.splits - 1, a.by_few_splits);
         t0 = t0 + split * share;
         t1 = min(t1, t0 + share);
     }
@@ -429,7 +427,7 @@ __device__ __forceinline__ void attn_rows(const AttnLaunch &a, RowsLds &lds, int
 
     const int o_row = tid / 16, o_d = tid % 16 * 4;  // what this thread writes of 64 dimensions
     const bool writes = row0 + o_row < rows;
-    const int o_t = writes ? (row0 + o_row) / a.group : 0, o_h = head * a.group + (writes ? row0 + o_row - o_t * a.group : 0);
+    const int o_t = writes ? divided(row0 + o_row, a.by_group) : 0, o_h = head * a.group + (writes ? row0 + o_row - o_t * a.group : 0);
     joined(o_row, top, base, sum);
     const int64_t index = ((int64_t)item * a.c.kv_heads + head) * a.few.splits + split;
     float *part = a.few.part + index * (ROWS * (DP + 2));
@@ -502,26 +500,26 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const int r = lane % 32, h = lane / 32;
     // heads fastest: with eight of them every XCD keeps one head's cache in its L2; later tiles (longer ones) first
-    const int rest = same(work, a.c.kv_heads), head = work - rest * a.c.kv_heads;
-    const int nth = same(rest, a.many.splits), split = rest - nth * a.many.splits, item = a.many.items - 1 - nth;
+    const int rest = divided(work, a.by_heads), head = work - rest * a.c.kv_heads;
+    const int nth = divided(rest, a.by_many_splits), split = rest - nth * a.many.splits, item = a.many.items - 1 - nth;
     Found at_item;
     if (!find_item(a.b, item, [&](int n, int) { return tiles_of<TILE>(a.many, a.group, n); }, at_item)) return;
     const int seq = at_item.seq, tile = at_item.local, begin = at_item.begin;
     const int n = at_item.n, len = at_item.len, first = len - n;
     const int rows = n * a.group, row0 = tile * TILE, wrow0 = row0 + 32 * wave;
     const bool valid = wrow0 + r < rows;
-    const int my_t = valid ? (wrow0 + r) / a.group : 0, my_h = valid ? wrow0 + r - my_t * a.group : 0;
+    const int my_t = valid ? divided(wrow0 + r, a.by_group) : 0, my_h = valid ? wrow0 + r - my_t * a.group : 0;
     int lo, hi, lo_min, lo_max, hi_min, hi_max, w_lo_min, w_lo_max, w_hi_min, w_hi_max;
     visible(a, first + my_t, len, lo, hi);
-    visible(a, first + same(row0, a.group), len, lo_min, hi_min);
-    visible(a, first + same(min(row0 + TILE, rows) - 1, a.group), len, lo_max, hi_max);
-    visible(a, first + same(min(wrow0, rows - 1), a.group), len, w_lo_min, w_hi_min);
-    visible(a, first + same(min(wrow0 + 32, rows) - 1, a.group), len, w_lo_max, w_hi_max);
+    visible(a, first + divided(row0, a.by_group), len, lo_min, hi_min);
+    visible(a, first + divided(min(row0 + TILE, rows) - 1, a.by_group), len, lo_max, hi_max);
+    visible(a, first + divided(min(wrow0, rows - 1), a.by_group), len, w_lo_min, w_hi_min);
+    visible(a, first + divided(min(wrow0 + 32, rows) - 1, a.by_group), len, w_lo_max, w_hi_max);
 
     // Everything that a tile waits for once is asked for as early as it can be: page numbers, queries, the first page.
     int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
     if (a.many.splits > 1) {
-        const int share = same(t1 - t0 + a.many.splits - 1, a.many.splits);
+        const int share = divided(t1 - t0 + a.many.splits - 1, a.by_many_splits);
         t0 = t0 + split * share;
         t1 = min(t1, t0 + share);
     }
@@ -832,8 +830,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnLaunch a) {
     const int64_t size = R * (dp + 2);
     const float *part = share.part + ((int64_t)blockIdx.x * a.c.kv_heads + head) * share.splits * size;
     for (int i = threadIdx.x + blockIdx.z * 256; i < rows * quads; i += 256 * gridDim.z) {
-        const int row = i / quads, d = (i - row * quads) * 4;
-        const int t = (tile * R + row) / a.group, h = head * a.group + tile * R + row - t * a.group;
+        const int row = divided(i, a.by_quads), d = (i - row * quads) * 4;
+        const int t = divided(tile * R + row, a.by_group), h = head * a.group + tile * R + row - t * a.group;
         float top = MINUS_INF, sum = 0.f;
         float4v y = {0.f, 0.f, 0.f, 0.f};
         const float sink = a.sinks ? a.sinks[h] * LOG2E : MINUS_INF;
@@ -975,9 +973,15 @@ size_t attn_workspace_floats(const DevKv &c, const DevBatch &b, const AttnDesc &
 hipError_t launch_attention(const DevKv &c, const DevBatch &b, const AttnDesc &d, const void *q, int64_t q_stride, void *out,
                             int64_t out_stride, float *workspace, int num_cus, hipStream_t s) {
     AttnLaunch a{c, b, q, out, q_stride, out_stride, d.n_heads, d.n_heads / c.kv_heads, d.scale, d.softcap, d.causal, d.window,
-                 d.sinks, c.block == 16 ? 0 : c.block == 32 ? 1 : 2, Share{}, Share{}};
+                 d.sinks, c.block == 16 ? 0 : c.block == 32 ? 1 : 2, Share{}, Share{}, {}, {}, {}, {}, {}, {}};
     size_t floats[2];
     shares_of(c, b, d, num_cus, a.few, a.many, floats);
+    a.by_group = divisor_of(a.group);
+    a.by_heads = divisor_of(c.kv_heads);
+    a.by_few_items = divisor_of(a.few.items ? a.few.items : 1);
+    a.by_few_splits = divisor_of(a.few.splits);
+    a.by_many_splits = divisor_of(a.many.splits);
+    a.by_quads = divisor_of(c.head_dim / 4);
     a.few.part = workspace;
     a.many.part = workspace + floats[0];
     if (d.type == T_F32) return launch_t<float>(a, s);

@@ -57,6 +57,22 @@ __device__ __forceinline__ int scan_add(int x) {
     return x;
 }
 
+// Division by a number that the host knows: 0 <= x < 2^31, 1 <= d < 2^31.  Three instructions, scalar ones where x is the
+// same for a wave; the general division is about forty vector instructions (and as much code to fetch).
+struct Divisor {
+    uint32_t mul, shift;
+};
+
+inline Divisor divisor_of(int64_t d) {
+    uint32_t shift = 0;
+    while ((int64_t(1) << shift) < d) shift++;
+    return Divisor{(uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - (uint64_t)d)) / (uint64_t)d + 1), shift};
+}
+
+__device__ __forceinline__ int divided(int x, const Divisor &d) {
+    return (int)((__umulhi((uint32_t)x, d.mul) + (uint32_t)x) >> d.shift);
+}
+
 // where a work item falls: its sequence, its number there, and the sequence's rows
 struct Found {
     int seq, local;

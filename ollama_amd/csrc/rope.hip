@@ -23,6 +23,7 @@ struct RopeLaunch {
     int64_t q_stride, k_stride, q_out_stride, k_out_stride;  // elements between rows
     const int32_t *pos;
     int n, chunks, heads_per_wave;
+    Divisor by_chunks;
 };
 
 template <int LPH>
@@ -37,8 +38,8 @@ template <class T, int LPH, bool HALVES>
 __global__ __launch_bounds__(256) void rope_kernel(RopeLaunch a) {
     using V4 = typename Vec4<T>::type;
     constexpr int GROUPS = 64 / LPH;
-    const int wave = (int)(blockIdx.x * 4 + threadIdx.x / 64), lane = threadIdx.x & 63;
-    const int row = wave / a.chunks, chunk = wave - row * a.chunks;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + threadIdx.x / 64)), lane = threadIdx.x & 63;
+    const int row = divided(wave, a.by_chunks), chunk = wave - row * a.chunks;
     if (row >= a.n) return;
     const RopeDesc &d = a.d;
     const int j = lane % LPH, rot_lanes = d.n_rot / 8;
@@ -131,6 +132,7 @@ hipError_t launch_t(RopeLaunch &a, hipStream_t s) {
     per = per < 1 ? 1 : per > steps ? steps : per;
     a.chunks = (int)((steps + per - 1) / per);
     a.heads_per_wave = (int)per * groups;
+    a.by_chunks = divisor_of(a.chunks);
     const int64_t waves = (int64_t)a.n * a.chunks;
     const dim3 grid((unsigned)((waves + 3) / 4));
     if (a.d.halves) rope_kernel<T, LPH, true><<<grid, 256, 0, s>>>(a);
@@ -150,7 +152,7 @@ hipError_t launch_d(RopeLaunch &a, hipStream_t s) {
 hipError_t launch_qk_norm_rope(int type, const RopeDesc &d, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
                                const int32_t *pos, int n, void *q_out, int64_t q_out_stride, void *k_out,
                                int64_t k_out_stride, hipStream_t s) {
-    RopeLaunch a{d, q, k, q_out, k_out, q_stride, k_stride, q_out_stride, k_out_stride, pos, n, 1, 1};
+    RopeLaunch a{d, q, k, q_out, k_out, q_stride, k_stride, q_out_stride, k_out_stride, pos, n, 1, 1, {}};
     if (type == T_F32) return launch_d<float>(a, s);
     if (type == T_F16) return launch_d<_Float16>(a, s);
     return launch_d<__bf16>(a, s);
