@@ -115,28 +115,33 @@ __device__ __forceinline__ void visible(const AttnLaunch &a, int pos, int len, i
     hi = max(hi, 0);
 }
 
-// cap(z) in units of log2 for N scores x / softcap: c log2(e) tanh(x).  Below 0.35 the odd series to x^11 (2e-8 of the value;
-// the formula with the exponential would lose eight bits there), and where no lane of the wave has more, that alone.
+// cap(z) in units of log2 for N scores x / softcap: c tanh(x), c = softcap log2(e).  Below 0.35 the odd series to x^11 (2e-8
+// of the value; the formula with the exponential loses eight bits there), and where no lane of the wave has more, that alone.
 template <int N>
 __device__ __forceinline__ void cap_scores(float (&x)[N], float c) {
-    float big = 0.f;
+    float big = 0.f, r[N];
 #pragma unroll
-    for (int i = 0; i < N; i++) big = fmaxf(big, fabsf(x[i]));
-    if (__ballot(!(big < 0.35f)) == 0) {
+    for (int i = 0; i < N; i++) {
+        big = fmaxf(big, fabsf(x[i]));
+        const float y = x[i] * x[i];
+        float p = __builtin_fmaf(y, -1382.f / 155925.f, 62.f / 2835.f);
+        p = __builtin_fmaf(y, p, -17.f / 315.f);
+        p = __builtin_fmaf(y, p, 2.f / 15.f);
+        p = __builtin_fmaf(y, p, -1.f / 3.f);
+        const float cx = c * x[i];
+        r[i] = __builtin_fmaf(cx * y, p, cx);
+    }
+    if (__ballot(!(big < 0.35f))) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const float y = x[i] * x[i];
-            float p = __builtin_fmaf(y, -1382.f / 155925.f, 62.f / 2835.f);
-            p = __builtin_fmaf(y, p, -17.f / 315.f);
-            p = __builtin_fmaf(y, p, 2.f / 15.f);
-            p = __builtin_fmaf(y, p, -1.f / 3.f);
-            const float cx = c * x[i];
-            x[i] = __builtin_fmaf(cx * y, p, cx);
+            // (1 - t) / (1 + t), t = exp(-2 |x|)
+            const float t = __builtin_amdgcn_exp2f(-2.f * LOG2E * fabsf(x[i]));
+            const float y = __builtin_copysignf(c * (1.f - t) * __builtin_amdgcn_rcpf(1.f + t), x[i]);
+            if (!(fabsf(x[i]) < 0.35f)) r[i] = y;
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] = c * tanhf(x[i]);
     }
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = r[i];
 }
 
 // Numbers of a sequence's pages, 64 at a time in the lanes of a register: pages from + step * (0 .. 63).  Neither they nor
