@@ -354,7 +354,7 @@ int mi_qmm_rope_freqs(int n_rot, double base, double freq_scale, double ext_fact
 /* A key/value cache in 8 bits: pages of MI_QMM_KV_PAGE tokens; one fp32 scale for keys and one for values per `block`
  * tokens (16, 32 or 64) and head.  The code of x is the whole number nearest to x / scale, -127..127.
  * memory NULL: the library allocates (and zeroes) the cache's device memory.  Otherwise it is the caller's, device memory
- * of mi_qmm_kv_bytes() bytes, 256-byte aligned, that outlives the handle: key codes, value codes, key scales, value
+ * of mi_qmm_kv_bytes() bytes, 256-byte aligned, that outlives the handle and is taken as it is: key codes, value codes, key scales, value
  * scales, one after the other.  With dp = head_dim rounded up to 64, codes are bytes of code + 128,
  * [n_pages][n_kv_heads][64 * dp], and lie inside a page and head at
  *     key   (token t, dimension d):  (((t / 16 * (dp / 64) + d / 64) * 4 + d % 64 / 16) * 16 + t % 16) * 16 + d % 16

@@ -215,6 +215,16 @@ __device__ __forceinline__ void take_out_nan(float (&ks)[4], float (&vs)[4], int
     }
 }
 
+// one past the last page that rows with these bounds see, of those that the table has
+__device__ __forceinline__ int last_page(const AttnLaunch &a, int t0, int lo_min, int hi_max) {
+    return hi_max > lo_min ? max(t0, min((hi_max - 1) / KV_PAGE + 1, a.b.max_pages)) : t0;
+}
+
+// the sum that a row starts with: NaN if it sees tokens behind the table's last page
+__device__ __forceinline__ float first_sum(const AttnLaunch &a, int lo, int hi) {
+    return hi > lo && (hi - 1) / KV_PAGE >= a.b.max_pages ? __builtin_nanf("") : 0.f;
+}
+
 // ---- 16 rows per workgroup: a step of few tokens --------------------------------------------------------------------
 // Bound: HBM (the cache is read once; 16 rows are worth 64 flops a byte).  A wave takes whole pages (64 tokens), the four
 // waves of a workgroup every fourth one, each with its own running maximum; the workgroup joins them, and where the
@@ -251,7 +261,7 @@ __device__ __forceinline__ void attn_rows(const AttnLaunch &a, RowsLds &lds, int
     visible(a, first + divided(min(row0 + ROWS, rows) - 1, a.by_group), len, lo_max, hi_max);
 
     // Everything that the rows wait for once is asked for as early as it can be: page numbers, queries, the first page.
-    int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
+    int t0 = lo_min / KV_PAGE, t1 = last_page(a, t0, lo_min, hi_max);
     if (a.few.splits > 1) {
         const int share = divided(t1 - t0 + a.few.splits - 1, a.by_few_splits);
         t0 = t0 + split * share;
@@ -329,7 +339,7 @@ __device__ __forceinline__ void attn_rows(const AttnLaunch &a, RowsLds &lds, int
     float4v acc[4 * NC];
 #pragma unroll
     for (int i = 0; i < 4 * NC; i++) acc[i] = float4v{0.f, 0.f, 0.f, 0.f};
-    float m = MINUS_INF, l = 0.f;
+    float m = MINUS_INF, l = first_sum(a, lo, hi);
     float ref = 0x1p-100f, unit = 0x1p115f;  // values are accumulated in units of ref * 2^-15 = 1 / unit
 
     for (int page = t0 + wave, k = 0; page < t1; page += 4, k++) {
@@ -522,7 +532,7 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
     visible(a, first + divided(min(wrow0 + 32, rows) - 1, a.by_group), len, w_lo_max, w_hi_max);
 
     // Everything that a tile waits for once is asked for as early as it can be: page numbers, queries, the first page.
-    int t0 = lo_min / KV_PAGE, t1 = hi_max > lo_min ? (hi_max + KV_PAGE - 1) / KV_PAGE : t0;
+    int t0 = lo_min / KV_PAGE, t1 = last_page(a, t0, lo_min, hi_max);
     if (a.many.splits > 1) {
         const int share = divided(t1 - t0 + a.many.splits - 1, a.by_many_splits);
         t0 = t0 + split * share;
@@ -617,7 +627,7 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
     for (int d = 0; d < 2 * NC; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[d][i] = 0.f;
-    float m = MINUS_INF, l = 0.f;
+    float m = MINUS_INF, l = first_sum(a, lo, hi);
     float ref = 0x1p-100f, unit = 0x1p109f;  // values are accumulated in units of ref * 2^-9 = 1 / unit
 
     for (int page = t0; page < t1; page++) {
@@ -888,7 +898,15 @@ hipError_t launch_one(const AttnLaunch &a, hipStream_t s) {
         const auto kernel = a.softcap > 0.f ? attn_tile_kernel<T, NC, true> : attn_tile_kernel<T, NC, false>;
         constexpr int lds = 2 * 4 * KV_PAGE * 64 * NC;
         static_assert(lds >= (int)sizeof(RowsLds), "the 16-row way shares the buffers");
-        if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if constexpr (lds > 65536) {
+            static bool allowed[2][64] = {};  // more than 64 KiB of dynamic LDS has to be allowed once per device
+            int dev = 0;
+            if (hipGetDevice(&dev) == hipSuccess && dev >= 0 && dev < 64 && !allowed[a.softcap > 0.f][dev]) {
+                const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+                if (e != hipSuccess) return e;
+                allowed[a.softcap > 0.f][dev] = true;
+            }
+        }
         kernel<<<few + many, 256, lds, s>>>(a);
     }
     hipError_t e = hipGetLastError();
@@ -953,8 +971,9 @@ void shares_of(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus
         }
         few.items = (int)items;
         few.splits = (int)(want < most ? want : most);
-        if (few.splits < 1) few.splits = 1;
         if (few.splits > 256) few.splits = 256;
+        if (items * c.kv_heads * few.splits > 65536) few.splits = (int)(65536 / (items * c.kv_heads));  // a GB of partial results
+        if (few.splits < 1) few.splits = 1;
         if (few.splits > 1) floats[0] = (size_t)items * c.kv_heads * few.splits * (ROWS * (size_t)(c.dp + 2));
     }
     if (some_many) {

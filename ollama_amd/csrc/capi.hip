@@ -2045,8 +2045,9 @@ int check_kv(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *b) {
     return MI_QMM_OK;
 }
 
-// host arrays are looked at: every page that the call needs exists; each written page belongs to one sequence
-int check_host_batch(const mi_qmm_kv *kv, const mi_qmm_batch *b, int64_t n, bool whole, bool writes) {
+// host arrays are looked at: every page that the call needs -- from `back` tokens before a sequence's first row on --
+// exists; each written page belongs to one sequence
+int check_host_batch(const mi_qmm_kv *kv, const mi_qmm_batch *b, int64_t n, int64_t back, bool writes) {
     uint8_t *seen = nullptr;
     if (writes) {
         seen = new (std::nothrow) uint8_t[(size_t)kv->dev.n_pages]();
@@ -2060,7 +2061,8 @@ int check_host_batch(const mi_qmm_kv *kv, const mi_qmm_batch *b, int64_t n, bool
         else if (len < 0 || len > (int64_t)b->max_pages * KV_PAGE || to - from > len)
             rc = fail(MI_QMM_ERR_INVALID, "sequence %d: %lld rows, %lld tokens, a table of %d pages", s, (long long)(to - from), (long long)len, b->max_pages);
         if (rc || to == from) continue;
-        for (int64_t p = whole ? 0 : (len - (to - from)) / KV_PAGE; p * KV_PAGE < len && !rc; p++) {
+        const int64_t first = len - (to - from) - back;
+        for (int64_t p = (first > 0 ? first : 0) / KV_PAGE; p * KV_PAGE < len && !rc; p++) {
             const int64_t page = b->pages[(int64_t)s * b->max_pages + p];
             if (page < 0 || page >= kv->dev.n_pages)
                 rc = fail(MI_QMM_ERR_INVALID, "sequence %d: page %lld is outside 0..%lld", s, (long long)page, (long long)kv->dev.n_pages - 1);
@@ -2239,7 +2241,7 @@ int mi_qmm_kv_write(mi_qmm_ctx *ctx, mi_qmm_kv *kv, const mi_qmm_batch *b, int t
     if ((rc = check_rows("k", k, k_stride, c.kv_heads, c.head_dim, type, location)) ||
         (rc = check_rows("v", v, v_stride, c.kv_heads, c.head_dim, type, location)))
         return rc;
-    if (location == MI_QMM_HOST && (rc = check_host_batch(kv, b, n, false, true))) return rc;
+    if (location == MI_QMM_HOST && (rc = check_host_batch(kv, b, n, 0, true))) return rc;
     const void *src[5];
     size_t bytes[5];
     batch_sources(b, src, bytes);
@@ -2261,7 +2263,7 @@ int mi_qmm_kv_read(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *b, 
     if ((rc = check_rows("k", k, k_stride, c.kv_heads, c.head_dim, type, location)) ||
         (rc = check_rows("v", v, v_stride, c.kv_heads, c.head_dim, type, location)))
         return rc;
-    if (location == MI_QMM_HOST && (rc = check_host_batch(kv, b, n, false, false))) return rc;
+    if (location == MI_QMM_HOST && (rc = check_host_batch(kv, b, n, 0, false))) return rc;
     const void *src[5];
     size_t bytes[5];
     batch_sources(b, src, bytes);
@@ -2294,7 +2296,7 @@ int mi_qmm_attention(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *b
     if ((rc = check_rows("q", q, q_stride, p->n_heads, c.head_dim, p->type, location)) ||
         (rc = check_rows("out", out, out_stride, p->n_heads, c.head_dim, p->type, location)))
         return rc;
-    if (location == MI_QMM_HOST && (rc = check_host_batch(kv, b, n, true, false))) return rc;
+    if (location == MI_QMM_HOST && (rc = check_host_batch(kv, b, n, p->window > 0 ? p->window - 1 : INT32_MAX, false))) return rc;
     const void *src[6];
     size_t bytes[6];
     batch_sources(b, src, bytes);

@@ -92,7 +92,7 @@ __device__ __forceinline__ bool find_item(const DevBatch &b, int item, F count, 
         if (s < b.n_seqs) {
             begin = b.row_start[s];
             const int end = b.row_start[s + 1];
-            len = b.kv_len[s];
+            len = max(b.kv_len[s], 0);
             n = begin >= 0 && end <= b.n_rows && end > begin ? end - begin : 0;
             c = count(n, len);
         }

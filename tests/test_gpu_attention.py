@@ -376,12 +376,86 @@ ATTEND = [  # lens, new rows, heads, kv_heads, dim, block, kind, options
     ([640], [300], 8, 2, 256, 64, "f16", {"cap": 50.0}),
     ([350], [130], 2, 2, 128, 64, "f32", {"spread": 40.0}),
     ([350], [130], 2, 2, 128, 64, "f16", {"spread": 1e-5, "scale": 1e4}),
+    ([300], [1], 64, 1, 64, 16, "f32", {}),                                       # one token of many heads per key head
+    ([8200, 300, 5000, 64], [1, 150, 2, 0], 4, 1, 64, 64, "f32", {}),             # prompts and single tokens, the latter split
+    ([4200, 40, 700], [3, 40, 300], 6, 2, 128, 32, "bf16", {"sinks": True}),
+    ([4200, 40, 700], [3, 40, 300], 2, 2, 256, 16, "f16", {"window": 200, "cap": 15.0}),
+    ([200, 90], [100, 1], 4, 4, 8, 64, "f32", {}),
+    ([200, 90], [100, 80], 4, 2, 24, 16, "bf16", {}),
+    ([333], [64], 8, 2, 200, 32, "f32", {"cap": 3.0}),
+    ([333], [64], 8, 2, 128, 32, "f32", {"scale": -0.2}),
+    ([333], [2], 8, 2, 128, 32, "f16", {"scale": -0.2}),
+    ([70, 333], [64, 1], 8, 2, 64, 32, "f32", {"scale": 1e-30}),
+    ([3000], [100], 1, 1, 256, 64, "f32", {}),
+    ([600, 500], [600, 500], 3, 1, 192, 64, "f32", {"sinks": True}),
 ]
 
 
 @pytest.mark.parametrize("lens,news,heads,kv_heads,dim,block,kind,options", ATTEND)
 def test_attention(ctx, lens, news, heads, kv_heads, dim, block, kind, options):
     _attend(ctx, np.random.default_rng(sum(lens) + dim), lens, news, heads, kv_heads, dim, block, kind, **options)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("block", [16, 64])
+def test_attention_of_scales_far_apart(ctx, kind, new, block):
+    """keys that grow along the sequence (the maximum leaves every reference behind), values whose scales differ by many
+    orders of magnitude from block to block in both directions, blocks of zeros among them"""
+    t, half = TYPES[kind]
+    rng = np.random.default_rng(block + new)
+    n, dim = 700, 64
+    k = rng.standard_normal((n, 1, dim)) * np.linspace(0.2, 6, n)[:, None, None]
+    v = rng.standard_normal((n, 1, dim))
+    for b in range(0, n, 64):
+        v[b:b + 64] *= 10.0 ** rng.uniform(-9, 3)
+    k[128:192], v[256:320], v[0:64] = 0, 0, 0
+    k, v = k.astype(np.float32), v.astype(np.float32)
+    ref = attnref.Cache(12, 1, dim, block)
+    pages = rng.permutation(12)[:11].reshape(1, 11)
+    kv = ctx.kv_create(12, 1, dim, block)
+    ctx.kv_write(kv, qmm.Batch.of([0, n], [n], pages), k, v)
+    ref.write([0, n], [n], pages, k, v)
+    with Device(ctx) as dev:
+        for sign in (1.0, -1.0):  # the keys of the end against the rows, and with them
+            q, qv = dev.values(rng.standard_normal((new, 3, dim)) + sign * k[-1], kind)
+            out = dev.values(np.zeros((new, 3, dim)), kind)[0]
+            b = qmm.Batch(1, 11, dev(np.array([0, new], np.int32)).ptr, dev(np.array([n], np.int32)).ptr, dev(pages, np.int32).ptr)
+            ctx.attention_device(kv, b, qmm.Attention(t, 3, 0.05), q.ptr, new, out.ptr)
+            ctx.sync()
+            want, bound = attnref.attention(ref, [0, new], [n], pages, qv, np.float64(np.float32(0.05)))
+            # what each row could take from its largest value, weighted: a rounding of a probability is one of its own share
+            got = host(out, kind)
+            bar = bound + (0 if kind == "f32" else np.abs(v).max() * 2.0 ** -10 + half * np.abs(want)) + 2.0 ** -24 * np.abs(want)
+            assert np.all(np.abs(got - want) <= bar)
+            if sign < 0:  # rows that turn from the large values to small ones: exact to the small ones' own size
+                assert np.isfinite(got).all()
+    kv.free()
+
+
+def test_attention_of_lengths_behind_the_table(ctx):
+    """device lengths beyond the page table, absurd and negative ones: NaN for the rows that see such tokens, zeros for rows
+    that see none, and the call ends"""
+    rng = np.random.default_rng(6)
+    for kind in ("f32", "f16"):
+        t, _ = TYPES[kind]
+        with Device(ctx) as dev:
+            kv = ctx.kv_create(4, 1, 64, 64)
+            k = rng.standard_normal((128, 1, 64)).astype(np.float32)
+            ctx.kv_write(kv, qmm.Batch.of([0, 128], [128], [[0, 1]]), k, k)
+            pages, n = dev(np.array([[0, 1]] * 5, np.int32)), 50
+            q = dev.values(rng.standard_normal((5 * n, 2, 64)), kind)[0]
+            for window in (0, 30):
+                out = dev.values(np.full((5 * n, 2, 64), 7.0), kind)[0]
+                lens = dev(np.array([128, 150, 2 ** 31 - 1, -7, -2 ** 31], np.int32))
+                b = qmm.Batch(5, 2, dev(np.arange(6) * n, np.int32).ptr, lens.ptr, pages.ptr)
+                ctx.attention_device(kv, b, qmm.Attention(t, 2, 0.125, window), q.ptr, 5 * n, out.ptr)
+                ctx.sync()
+                got = host(out, kind).reshape(5, n, -1)
+                assert np.isfinite(got[0]).all() and not (got[0] == 0).all(-1).any()
+                assert np.isfinite(got[1, :28]).all() and np.isnan(got[1, 28:]).all()  # row 28 is at position 128
+                assert np.isnan(got[2]).all() and np.all(got[3:] == 0)
+            kv.free()
 
 
 def test_attention_rows_that_see_nothing(ctx):
@@ -490,6 +564,11 @@ def test_refusals(ctx):
         assert L.mi_qmm_kv_read(ctx._h, kv._h, b._p, qmm.F32, a.ptr, 128, a.ptr + 256, 128, 2, qmm.DEVICE) == qmm.ERR_INVALID
         none = qmm.Batch(0, 1, None, None, None)
         assert L.mi_qmm_attention(ctx._h, kv._h, none._p, how._p, a.ptr, 256, o.ptr, 256, 2, qmm.DEVICE) == 0
+    # pages that a window leaves behind may be gone
+    far = qmm.Batch.of([0, 10], [128], [[-1, 2]])
+    assert ctx.attention(kv, far, q, 1.0, window=55).shape == q.shape
+    with pytest.raises(qmm.QmmError):
+        ctx.attention(kv, far, q, 1.0, window=56)
     kv.free()
 
 
@@ -588,6 +667,41 @@ def test_steps_replayed_from_a_graph(ctx):
                     own.attention_device(kv, wide, big, qb.ptr, 3, ob.ptr)
             assert "frozen" in str(e.value)
             own.scratch_freeze(False)
+            kv.free()
+    finally:
+        own.set_stream(None)
+        own.close()
+        stream.destroy()
+
+
+def test_prompts_replayed_from_a_graph(ctx):
+    """the 128-row way with split tiles at heads of 256, captured: every replay the eager bits, with eager work between"""
+    rng = np.random.default_rng(22)
+    own = qmm.Context(0)
+    stream = Stream()
+    own.set_stream(stream.ptr.value)
+    try:
+        with Device(own) as dev:
+            kv = own.kv_create(20, 2, 256, 32)
+            pages = rng.permutation(20)[:16].reshape(1, 16).astype(np.int32)
+            k, v = rng.standard_normal((2, 1000, 2, 256)).astype(np.float32)
+            own.kv_write(kv, qmm.Batch.of([0, 1000], [1000], pages), k, v)
+            q, out = dev(rng.standard_normal((90, 4, 256)).astype(np.float32)), dev(np.zeros((90, 4, 256), np.float32))
+            b = qmm.Batch(1, 16, dev(np.array([0, 90], np.int32)).ptr, dev(np.array([1000], np.int32)).ptr, dev(pages).ptr)
+            how = qmm.Attention(qmm.F32, 4, 0.0625, softcap=20.0)
+            step = lambda: own.attention_device(kv, b, how, q.ptr, 90, out.ptr)  # noqa: E731
+            step()
+            stream.sync()
+            replay = stream.capture(step)
+            for i in range(4):
+                q.set(rng.standard_normal((90, 4, 256)).astype(np.float32))
+                step()
+                stream.sync()
+                want = out.numpy()
+                out.set(np.zeros(out.shape, np.float32))
+                assert replay() == 0
+                stream.sync()
+                assert np.array_equal(out.numpy(), want) and np.abs(want).max() > 0
             kv.free()
     finally:
         own.set_stream(None)
