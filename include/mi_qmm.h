@@ -321,8 +321,9 @@ int mi_qmm_mulmat_id_produced(mi_qmm_ctx *ctx, const mi_qmm_weight *w, int n_exp
  *      Rotation, cache and attention take activations of type MI_QMM_TYPE_F32, _F16 or _BF16 (the products' own are f32);
  *      sums, softmax statistics and norms are fp32 and every result is rounded once.  Row pointers are 16-byte aligned
  *      and row strides (elements from one row to the next, at least a row's values) whole 16-byte pieces in bytes;
- *      head_dim is a multiple of 8 up to 256; a call has at most 2^22 rows, attention 2^27 rows times heads; anything else is MI_QMM_ERR_INVALID or _UNSUPPORTED.  `location` covers
- *      every pointer of a call, those inside the structs included; a cache is always device memory. */
+ *      head_dim is a multiple of 8 up to 256; a call has at most 2^22 rows, attention at most 2^27 in n * n_heads +
+ *      15 * min(n, n_seqs) * n_kv_heads; anything else is MI_QMM_ERR_INVALID or _UNSUPPORTED.  `location` covers every
+ *      pointer of a call, those inside the structs included; a cache is always device memory. */
 
 /* Norms of queries and keys for each head and the rotation by position, in one pass:
  *     y = x / sqrt(mean(x^2) + eps) * weight     over the head_dim values of a head; left out where the weight is NULL
@@ -396,9 +397,12 @@ int mi_qmm_kv_read(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *bat
  *     out = sum_j w_j v_j / (sum_j w_j + exp(sink)),  w_j = exp(z_j),  z_j = cap(scale * q . k_j),  cap(z) = c tanh(z / c)
  * over the tokens j of the row's sequence with j <= its position (causal) and j > its position - window (window > 0).
  * Query head h reads key/value head h / (n_heads / n_kv_heads).  sinks: one logit per query head that takes part in the
- * sum only; softcap 0: no cap.  A row that sees no token gives zeros.  f32 calls carry f32 accuracy (queries and
- * probabilities are split into two halves each); the 16-bit types take probabilities of 11 bits.  The rows' own tokens
- * are to be written first (mi_qmm_kv_write on the same batch).  q, out [n][n_heads][head_dim], not overlapping. */
+ * sum only; softcap 0: no cap; scale and softcap are finite.  A row that sees no token gives zeros.  f32 calls carry f32
+ * accuracy (queries and probabilities are split into two halves each); the 16-bit types take probabilities of 11 bits
+ * (f16 of 22).  A value's share (its weight times its scale) is rounded at 2^-34 of the largest value scale among the
+ * tokens that the 128 (token, head) rows worked on together see, so scales that far apart do not add up to f32 accuracy.
+ * The rows' own tokens are to be written first (mi_qmm_kv_write on the same batch).  q, out [n][n_heads][head_dim], not
+ * overlapping. */
 typedef struct mi_qmm_attn {
     int type, n_heads;
     float scale, softcap;

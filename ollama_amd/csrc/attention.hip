@@ -162,9 +162,11 @@ __device__ __forceinline__ float lane_float(float x, int lane) {
     return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), lane));
 }
 
-// as scalars; NaN where there is no such page: whoever sees it gets NaN
-__device__ __forceinline__ void spread_scales(float x, int phys, float (&ks)[4], float (&vs)[4]) {
-    x = phys < 0 ? __builtin_nanf("") : x;
+// as scalars; NaN where there is no such page: whoever sees it gets NaN.  Scales of 16 tokens that none of the rows worked on
+// together (lo .. hi - 1 for all of them) sees are 0: what stands there is a page's earlier content, and of any size.
+__device__ __forceinline__ void spread_scales(float &x, int phys, int j0, int lo, int hi, float (&ks)[4], float (&vs)[4]) {
+    const int j = j0 + 16 * (threadIdx.x & 3);
+    x = j < hi && j + 16 > lo ? (phys < 0 ? __builtin_nanf("") : x) : 0.f;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
         ks[t] = lane_float(x, t);
@@ -348,8 +350,8 @@ __device__ __forceinline__ void attn_rows(const AttnLaunch &a, RowsLds &lds, int
             fetch(phys);
         }
         float ks[4], vs[4];
-        spread_scales(sc, phys, ks, vs);
         const int j0 = page * KV_PAGE;
+        spread_scales(sc, phys, j0, lo_min, hi_max, ks, vs);
         take_out_nan(ks, vs, j0, lo, hi, l);
         float z[16];
 #pragma unroll
@@ -643,8 +645,8 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
     for (int page = t0; page < t1; page++) {
         const int b = (page - t0) & 1;
         lds_barrier();
-        spread_scales(sc, phys, ks, vs);
         const int j0 = page * KV_PAGE;
+        spread_scales(sc, phys, j0, w_lo_min, w_hi_max, ks, vs);
         const bool works = wrow0 < rows && j0 < w_hi_max && j0 + KV_PAGE > w_lo_min;  // else nothing that this wave's rows see
         if (works) {
         take_out_nan(ks, vs, j0, lo, hi, l);

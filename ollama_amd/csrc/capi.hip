@@ -2291,7 +2291,11 @@ int mi_qmm_attention(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *b
     if (p->n_heads < 1 || p->n_heads > 65535 || p->n_heads % c.kv_heads)
         return fail(MI_QMM_ERR_INVALID, "n_heads=%d is no multiple of the cache's %d heads", p->n_heads, c.kv_heads);
     if (!(p->softcap >= 0.f) || p->window < 0) return fail(MI_QMM_ERR_INVALID, "softcap=%g window=%d must be non-negative", (double)p->softcap, p->window);
-    if (n * p->n_heads > (1 << 27)) return fail(MI_QMM_ERR_UNSUPPORTED, "n=%lld rows of %d heads", (long long)n, p->n_heads);
+    if (!std::isfinite(p->scale) || !std::isfinite(p->softcap))
+        return fail(MI_QMM_ERR_INVALID, "scale=%g softcap=%g must be finite", (double)p->scale, (double)p->softcap);
+    // a launch has at most 2^24 workgroups of 256: 16 rows each, one more per sequence and head
+    if (n * p->n_heads + 15 * std::min<int64_t>(n, b->n_seqs) * c.kv_heads > (1 << 27))
+        return fail(MI_QMM_ERR_UNSUPPORTED, "n=%lld rows of %d heads in %d sequences", (long long)n, p->n_heads, b->n_seqs);
     if (n == 0 || b->n_seqs == 0) return MI_QMM_OK;
     if ((rc = check_rows("q", q, q_stride, p->n_heads, c.head_dim, p->type, location)) ||
         (rc = check_rows("out", out, out_stride, p->n_heads, c.head_dim, p->type, location)))

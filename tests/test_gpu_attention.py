@@ -433,6 +433,43 @@ def test_attention_of_scales_far_apart(ctx, kind, new, block):
     kv.free()
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("news", [(1, 2, 1), (40, 70, 1), (100, 120, 200)])
+@pytest.mark.parametrize("dim,block", [(64, 16), (128, 32), (200, 64)])
+def test_attention_over_memory_with_earlier_content(ctx, kind, news, dim, block):
+    """a cache in memory that is not cleared: codes and scales of any size, infinities and NaN stand behind the last token
+    and in tokens that a window has left, and no result changes by a bit"""
+    t, half = TYPES[kind]
+    rng = np.random.default_rng(dim + sum(news))
+    lens, pages = [101, 130, 200], rng.permutation(12).reshape(3, 4).astype(np.int32)
+    rs = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    starts = np.concatenate([[0], np.cumsum(news)]).astype(np.int32)
+    k, v = rng.standard_normal((2, 431, 2, dim)).astype(np.float32)
+    size, codes = qmm.kv_bytes(12, 2, dim, block), 2 * 12 * 2 * 64 * attnref.row_dim(dim)
+    used = rng.integers(0, 256, size).astype(np.uint8)
+    scales = rng.choice(np.array([3e38, np.inf, np.nan, 1e30, -1e20, 1e-44, 5e3, -np.inf], np.float32), (size - codes) // 4)
+    used[codes:] = scales.view(np.uint8)
+    ref = attnref.Cache(12, 2, dim, block)
+    ref.write(rs, lens, pages, k, v)
+    got = []
+    with Device(ctx) as dev:
+        q, qv = dev.values(rng.standard_normal((int(starts[-1]), 6, dim)), kind)
+        for memory in (np.zeros(size, np.uint8), used):
+            kv = ctx.kv_create(12, 2, dim, block, memory=dev(memory).ptr)
+            ctx.kv_write(kv, qmm.Batch.of(rs, lens, pages), k, v)
+            b = qmm.Batch(3, 4, dev(starts, np.int32).ptr, dev(np.array(lens, np.int32)).ptr, dev(pages).ptr)
+            for window, cap in ((0, 0.0), (90, 20.0)):
+                out = dev.values(np.zeros((int(starts[-1]), 6, dim)), kind)[0]
+                ctx.attention_device(kv, b, qmm.Attention(t, 6, 0.2, window, cap), q.ptr, int(starts[-1]), out.ptr)
+                ctx.sync()
+                got.append(host(out, kind))
+                want, bound = attnref.attention(ref, starts, lens, pages, qv, np.float64(np.float32(0.2)), window, cap)
+                bar = bound + (0 if kind == "f32" else np.abs(v).max() * 2.0 ** -10 + half * np.abs(want)) + 2.0 ** -24 * np.abs(want)
+                assert np.all(np.abs(got[-1] - want) <= bar)
+            kv.free()
+    assert np.array_equal(got[0], got[2]) and np.array_equal(got[1], got[3])
+
+
 def test_attention_of_lengths_behind_the_table(ctx):
     """device lengths beyond the page table, absurd and negative ones: NaN for the rows that see such tokens, zeros for rows
     that see none, and the call ends"""
@@ -547,6 +584,10 @@ def test_refusals(ctx):
         ctx.attention(kv, ok, q, 1.0, softcap=-1.0)
     with pytest.raises(qmm.QmmError):
         ctx.attention(kv, ok, q, 1.0, window=-1)
+    for bad in ({"scale": np.nan}, {"scale": np.inf}, {"scale": 1.0, "softcap": np.inf}):
+        with pytest.raises(qmm.QmmError) as e:
+            ctx.attention(kv, ok, q, **bad)
+        assert e.value.code == qmm.ERR_INVALID
     with pytest.raises(ValueError):
         ctx.attention(kv, ok, np.zeros((10, 4, 128), np.float32), 1.0)
     L = qmm.lib()
