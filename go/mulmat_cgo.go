@@ -120,6 +120,32 @@ func (c *Context) Compute(ts ...*Tensor) {
 	}
 }
 
+// KVCache is one layer's key/value cache in 8 bits (mi_qmm_kv_create): pages of MI_QMM_KV_PAGE tokens of device memory.
+type KVCache struct {
+	b  *Backend
+	kv *C.mi_qmm_kv
+}
+
+func (b *Backend) newKVCache(pages int64, kvHeads, headDim, block int) *KVCache {
+	c := &KVCache{b: b}
+	check(C.mi_qmm_kv_create(b.ctx, C.int64_t(pages), C.int(kvHeads), C.int(headDim), C.int(block), nil, &c.kv))
+	return c
+}
+
+func (c *KVCache) free() { C.mi_qmm_kv_free(c.kv) }
+
+// step binds a layer's calls between the q / k / v products and the o product, all on the ctx's stream: rotation in place,
+// the rows into the cache, attention.  q, k, v, out are device addresses of f32 rows without gaps, pos the rows'
+// positions on the device; batch holds device addresses (row starts, lengths, page tables) and is C memory, as are heads
+// (with its frequencies, which mi_qmm_rope_freqs fills, and its norm weights on the device) and how.
+func (c *KVCache) step(heads *C.mi_qmm_qk_heads, batch *C.mi_qmm_batch, how *C.mi_qmm_attn, q, k, v, out unsafe.Pointer,
+	pos *C.int32_t, n int64) {
+	qs, ks := C.int64_t(heads.n_heads*heads.head_dim), C.int64_t(heads.n_kv_heads*heads.head_dim)
+	check(C.mi_qmm_qk_norm_rope(c.b.ctx, heads, q, qs, k, ks, pos, C.int64_t(n), q, qs, k, ks, C.MI_QMM_DEVICE))
+	check(C.mi_qmm_kv_write(c.b.ctx, c.kv, batch, heads._type, k, ks, v, ks, C.int64_t(n), C.MI_QMM_DEVICE))
+	check(C.mi_qmm_attention(c.b.ctx, c.kv, batch, how, q, qs, out, qs, C.int64_t(n), C.MI_QMM_DEVICE))
+}
+
 // quantizeTensor binds mi_qmm_quantize_weights: the per-tensor step of quantize(), which the reference hands to the
 // external llama-quantize (server/quantization.go:125-181, called from server/create.go:931-944).
 func (b *Backend) quantizeTensor(typ uint32, rows []float32, k, m int) []byte {

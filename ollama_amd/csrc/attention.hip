@@ -230,6 +230,9 @@ __device__ __forceinline__ float first_sum(const AttnLaunch &a, int lo, int hi) 
 // Bound: HBM (the cache is read once; 16 rows are worth 64 flops a byte).  A wave takes whole pages (64 tokens), the four
 // waves of a workgroup every fourth one, each with its own running maximum; the workgroup joins them, and where the
 // cache is split over workgroups a second kernel joins those.
+//
+// Measured, f32, 32 query and 8 key/value heads of 128: 64 sequences of up to 8192 tokens 154 us (754 MB, 4.9 TB/s; a copy
+// runs at 5.4); one sequence of 4096 tokens 7.2 us and 3.5 us for the second kernel.
 constexpr int ROWS = 16;
 
 struct RowsLds {
@@ -501,9 +504,16 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
 
 // ---- 128 rows per workgroup: prompts ----------------------------------------------------------------------------------
 // Bound: the vector ALU beside the matrix cores.  A wave holds 32 rows, the workgroup's four waves share each page of 64
-// tokens through LDS (two buffers, loaded straight into them while the page before is worked on).  Per page and wave of 32
-// rows at a head of 128 the matrix cores have 1024 cycles of work; widening the codes and the softmax of 2048 scores, a
-// quarter-rate exponential each, are about twice that.
+// tokens through LDS: each widens a quarter of the codes, once for all 128 rows, while the matrix instructions of the page
+// before run (two buffers; the codes are in registers one page ahead of that).  The exponentials of the softmax and the
+// widening take the vector ALU about as long as the products take the matrix cores, and two waves per SIMD hide only part
+// of one behind the other: the 1024 scores of 32 rows against 32 tokens alone are 16 matrix instructions (538 ns) and 128
+// vector instructions (289 ns), and both together measured 720 ns.
+//
+// Measured: 2 prompts of 4096 and 2506 tokens, bf16, 32 and 8 heads of 128: 245-253 us = 760-780 TFLOP/s (569 us the 16-row
+// way, which widens every code for 16 rows at a time); 2048 rows over 32768 tokens 860 TFLOP/s; a large library product
+// runs at 1200.  f32, whose products are taken twice: 509 rows over 16001 tokens, 16 and 8 heads of 256, capped, 367 us =
+// 358 TFLOP/s (715 executed; 333 us without the cap).
 constexpr int TILE = 128;
 constexpr float LAZY = 6.f;
 
@@ -842,61 +852,102 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLau
     else attn_tile<T, NC, CAP>(a, lds, (int)blockIdx.x - few);
 }
 
-// The splits of a tile joined.  Bound by the latency of its three dependent rounds of loads (which sequence, the partial
-// results, the sinks): a thread takes four dimensions of one row and asks for eight splits' numerators and sums at a time,
-// before it knows their maximum.
-template <class T, int R>
+// The splits of a tile joined.  Bound by the latency of its dependent rounds of loads (which sequence, then the partial
+// results): a thread takes four dimensions of a row and asks for eight splits' maxima, sums and numerators at a time; where
+// that leaves the device empty, G = 8 threads share the splits and join through LDS (a row over 32768 tokens in 128 splits, the whole call: 38.2 us
+// with one thread, 24.3 with eight; 512 rows in two splits: 27.6 with one, 55.2 with eight).
+template <class T, int R, int G>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnLaunch a) {
+    constexpr int W = 256 / G;
+    __shared__ float4v lds_y[G > 1 ? G : 1][G > 1 ? W : 1];
+    __shared__ float lds_m[G > 1 ? G : 1][G > 1 ? W : 1], lds_l[G > 1 ? G : 1][G > 1 ? W : 1];
     const Share &share = R == ROWS ? a.few : a.many;
     using V4 = typename Vec4<T>::type;
-    const int head = blockIdx.y, dp = a.c.dp, quads = a.c.head_dim / 4;
+    const int head = blockIdx.y, dp = a.c.dp, quads = a.c.head_dim / 4, w = threadIdx.x % W, g = threadIdx.x / W;
     Found at_item;
     if (!find_item(a.b, (int)blockIdx.x, [&](int n, int) { return tiles_of<R>(share, a.group, n); }, at_item)) return;
     const int tile = at_item.local, begin = at_item.begin, n = at_item.n;
     const int rows = min(R, n * a.group - tile * R);
     const int64_t size = R * (dp + 2);
     const float *part = share.part + ((int64_t)blockIdx.x * a.c.kv_heads + head) * share.splits * size;
-    for (int i = threadIdx.x + blockIdx.z * 256; i < rows * quads; i += 256 * gridDim.z) {
-        const int row = divided(i, a.by_quads), d = (i - row * quads) * 4;
+    for (int i0 = blockIdx.z * W; i0 < rows * quads; i0 += gridDim.z * W) {
+        const int i = i0 + w;
+        const bool live = i < rows * quads;
+        const int row = live ? divided(i, a.by_quads) : 0, d = live ? (i - row * quads) * 4 : 0;
         const int t = divided(tile * R + row, a.by_group), h = head * a.group + tile * R + row - t * a.group;
+        const float sink = a.sinks ? a.sinks[h] * LOG2E : MINUS_INF;
         float top = MINUS_INF, sum = 0.f;
         float4v y = {0.f, 0.f, 0.f, 0.f};
-        const float sink = a.sinks ? a.sinks[h] * LOG2E : MINUS_INF;
-        for (int s0 = 0; s0 < share.splits; s0 += 8) {
-            float m[8], l[8];
-            float4v x[8];
+        // what a further part of the row adds: maximum m, sum l, numerators x; one that saw nothing has no numerators
+        auto add = [&](float base, float m, float l, const float4v &x) {
+            if (l == 0.f) return;
+            const float f = __builtin_amdgcn_exp2f(m - base);
+            sum += l * f;
 #pragma unroll
-            for (int s = 0; s < 8; s++) {
-                const float *p = part + min(s0 + s, share.splits - 1) * size;
-                m[s] = p[R * dp + row];
-                l[s] = p[R * dp + R + row];
-                x[s] = *(const float4v *)(p + row * dp + d);
-            }
-            float best = top;
+            for (int e = 0; e < 4; e++) y[e] += x[e] * f;
+        };
+        if (live) {
+            for (int s0 = g; s0 < share.splits; s0 += 8 * G) {
+                float m[8], l[8];
+                float4v x[8];
 #pragma unroll
-            for (int s = 0; s < 8; s++) best = fmaxf(best, m[s]);
-            const float base = best == MINUS_INF ? 0.f : best, keep = __builtin_amdgcn_exp2f(top - base);
-            top = best;
-            sum *= keep;
+                for (int s = 0; s < 8; s++) {
+                    const float *p = part + min(s0 + G * s, share.splits - 1) * size;
+                    m[s] = p[R * dp + row];
+                    l[s] = p[R * dp + R + row];
+                    x[s] = *(const float4v *)(p + row * dp + d);
+                }
+                float best = top;
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] *= keep;
+                for (int s = 0; s < 8; s++) best = fmaxf(best, m[s]);
+                const float base = best == MINUS_INF ? 0.f : best, keep = __builtin_amdgcn_exp2f(top - base);
+                top = best;
+                sum *= keep;
 #pragma unroll
-            for (int s = 0; s < 8; s++) {
-                if (s0 + s >= share.splits || l[s] == 0.f) continue;  // a split that saw nothing has no numerators
-                const float w = __builtin_amdgcn_exp2f(m[s] - base);
-                sum += l[s] * w;
+                for (int e = 0; e < 4; e++) y[e] *= keep;
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[e] += x[s][e] * w;
+                for (int s = 0; s < 8; s++)
+                    if (s0 + G * s < share.splits) add(base, m[s], l[s], x[s]);
             }
         }
-        // the sink joins the sum; where it is the largest, everything is measured against it
-        const float all = fmaxf(top == MINUS_INF ? 0.f : top, sink), scale = __builtin_amdgcn_exp2f((top == MINUS_INF ? 0.f : top) - all);
-        const float total = sum * scale + (a.sinks ? __builtin_amdgcn_exp2f(sink - all) : 0.f);
-        V4 w;
+        if constexpr (G > 1) {
+            lds_m[g][w] = top;
+            lds_l[g][w] = sum;
+            lds_y[g][w] = y;
+            __syncthreads();
+            if (g == 0) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = (T)(sum == 0.f ? 0.f : y[e] * scale / total);
-        *(V4 *)((T *)a.out + (int64_t)(begin + t) * a.out_stride + (int64_t)h * a.c.head_dim + d) = w;
+                for (int s = 0; s < G; s++) top = fmaxf(top, lds_m[s][w]);
+                sum = 0.f;
+                y = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < G; s++) add(top == MINUS_INF ? 0.f : top, lds_m[s][w], lds_l[s][w], lds_y[s][w]);
+            }
+        }
+        if (g == 0 && live) {
+            top = top == MINUS_INF ? 0.f : top;
+            // the sink joins the sum; where it is the largest, everything is measured against it
+            const float all = fmaxf(top, sink), scale = __builtin_amdgcn_exp2f(top - all);
+            const float total = sum * scale + (a.sinks ? __builtin_amdgcn_exp2f(sink - all) : 0.f);
+            V4 o;
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = (T)(sum == 0.f ? 0.f : y[e] * scale / total);
+            *(V4 *)((T *)a.out + (int64_t)(begin + t) * a.out_stride + (int64_t)h * a.c.head_dim + d) = o;
+        }
+        if (G > 1) __syncthreads();
     }
+}
+
+template <class T, int R>
+hipError_t launch_join(const AttnLaunch &a, const Share &share, hipStream_t s) {
+    // as many workgroups as the rows that a sequence has on average want; one with more of them goes round
+    const int64_t rows = ((int64_t)a.b.n_rows * a.group + a.b.n_seqs - 1) / a.b.n_seqs, values = (rows < R ? rows : R) * (a.c.head_dim / 4);
+    const auto grid = [&](int width) { return dim3((unsigned)share.items, (unsigned)a.c.kv_heads, (unsigned)((values + width - 1) / width)); };
+    // eight threads for each value where one would not fill the device (two tiles of 8 heads in ten splits: 62.9 us the whole
+    // call with eight threads, 55.7 with one; 16 single tokens in five splits 27.0 and 28.6)
+    if (values * share.items * a.c.kv_heads > 65536) attn_join_kernel<T, R, 1><<<grid(256), 256, 0, s>>>(a);
+    else attn_join_kernel<T, R, 8><<<grid(32), 256, 0, s>>>(a);
+    return hipGetLastError();
 }
 
 template <class T, int NC>
@@ -922,14 +973,8 @@ hipError_t launch_one(const AttnLaunch &a, hipStream_t s) {
         kernel<<<few + many, 256, lds, s>>>(a);
     }
     hipError_t e = hipGetLastError();
-    if (e == hipSuccess && few && a.few.splits > 1) {
-        attn_join_kernel<T, ROWS><<<dim3((unsigned)a.few.items, (unsigned)a.c.kv_heads), 256, 0, s>>>(a);
-        e = hipGetLastError();
-    }
-    if (e == hipSuccess && many && a.many.splits > 1) {  // 256 threads take 8 rows of 128: a tile is given to 16 workgroups
-        attn_join_kernel<T, TILE><<<dim3((unsigned)a.many.items, (unsigned)a.c.kv_heads, 16), 256, 0, s>>>(a);
-        e = hipGetLastError();
-    }
+    if (e == hipSuccess && few && a.few.splits > 1) e = launch_join<T, ROWS>(a, a.few, s);
+    if (e == hipSuccess && many && a.many.splits > 1) e = launch_join<T, TILE>(a, a.many, s);
     return e;
 }
 
@@ -944,15 +989,23 @@ hipError_t launch_t(const AttnLaunch &a, hipStream_t s) {
 }
 
 // Sequences of at most FEW (token, head) rows per key/value head go the 16-row way, longer ones the 128-row way.
-constexpr int FEW = 32;
+// Measured, 8 key/value heads of 128, f32: 16 sequences of 64 / 96 / 128 rows over up to 4096 tokens 54 / 76 / 86 us the 16-row
+// way, 72 / 77 / 82 the other; one sequence over 32768 tokens 44 / 65 / 77 and 49 / 51 / 54.
+constexpr int FEW = 64;
 
-// Workgroups that share a tile's cache, for `work` without and `slots` that run at a time.  Tiles that fill the device are
-// not split (a split tile's partial results are written and read once more, at 128 rows a third of the kernel's own time on
-// prompts of 4096); fewer are, so that they fill it, while a split keeps four pages.
-int splits_for(int64_t work, int64_t slots, int64_t pages) {
-    int64_t s = slots / work;
-    if (s > pages / 4) s = pages / 4;
-    return s < 1 ? 1 : s > 32 ? 32 : (int)s;
+// Workgroups that share a tile's cache of `pages` pages, of at most `most` that run at a time for each tile: where a page's
+// time (1.2 us at heads of 128, double for f32) over the split's pages, and behind it the joining launch (4 us) and the
+// partial results of all rows of the call written and read (`bytes` per split, at 4 TB/s) are least.  32 / 8 heads of 128,
+// bf16: 512 rows over their own 512 tokens 21.4 us in one piece, 27.6 in two, 32.3 in four; 64 over 1000 33.6 / 20.1 / 19.5
+// in 1 / 4 / 8 pieces; heads of 256, f32: 512 over 512 52.7 / 47.8 / 40.2 in 1 / 2 / 4.
+int splits_for(int64_t most, int64_t pages, double page_us, double bytes) {
+    int best = 1;
+    double least = pages * page_us;
+    for (int s = 2; s <= most && s <= pages && s <= 32; s++) {
+        const double us = (double)((pages + s - 1) / s) * page_us + 4.0 + s * (2.0 * bytes / 4e6);
+        if (us < least) { least = us; best = s; }
+    }
+    return best;
 }
 
 // Both shares with their splits; part is left to the caller.  floats: the partial results of each.
@@ -966,6 +1019,8 @@ void shares_of(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus
         const int64_t w = d.window > 0 && d.causal ? (d.window + rows) / KV_PAGE + 2 : b.max_pages;
         return w < b.max_pages ? w : (int64_t)b.max_pages;
     };
+    // tiles if the rows are spread evenly (items is what there can be at most: for 16 sequences of 128 rows twice as many)
+    auto likely = [&](int tile, int64_t seqs) { return seqs * ((all + seqs * tile - 1) / (seqs * tile)); };
     // a row per sequence, or few in all: the 16-row way; one sequence: either; otherwise a launch looks for both
     const bool some_many = all > FEW && b.n_rows > b.n_seqs, some_few = b.n_seqs > 1 || !some_many;
     if (some_few) {
@@ -978,8 +1033,10 @@ void shares_of(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus
             // and up to that length no second launch has to join anything
             want = (pages_seen(ROWS) + 63) / 64;
         } else {
-            // about eight workgroups per CU (rounds of them even out sequences of different lengths), down to a page per wave
-            want = 8ll * num_cus / (items * c.kv_heads) + 1;
+            // the workgroups that run at a time (three per CU at heads of 64, else two), down to a page per wave.  f32, 8
+            // heads of 128, two / eight per CU: one sequence of 32768 tokens 21.2 / 24.3 us, of 131072 49.8 / 55.5; 16 of up
+            // to 4096 tokens in 3 / 4 / 5 splits 31.1 / 27.0 / 29.9, 32 of up to 8192 in 1 / 2 / 3 80.9 / 83.8 / 88.3
+            want = (c.dp <= 64 ? 3ll : 2ll) * num_cus / (likely(ROWS, active) * c.kv_heads);
         }
         few.items = (int)items;
         few.splits = (int)(want < most ? want : most);
@@ -992,7 +1049,8 @@ void shares_of(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus
         const int64_t seqs = all / (FEW + 1) < active ? all / (FEW + 1) : active;  // sequences that can be longer than FEW
         many.items = (int)((all + (TILE - 1) * seqs) / TILE);
         if (b.n_seqs > 1) many.least = FEW + 1;
-        many.splits = splits_for((int64_t)many.items * c.kv_heads, (c.dp <= 128 ? 2 : 1) * num_cus, pages_seen(TILE));
+        many.splits = splits_for((c.dp <= 128 ? 2 : 1) * num_cus / (likely(TILE, seqs) * c.kv_heads), pages_seen(TILE),
+                                 c.dp / 128.0 * (d.type == T_F32 ? 2.4 : 1.2), 4.0 * (c.dp + 2) * b.n_rows * d.n_heads);
         if (many.splits > 1) floats[1] = (size_t)many.items * c.kv_heads * many.splits * (TILE * (size_t)(c.dp + 2));
     }
 }

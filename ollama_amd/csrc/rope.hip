@@ -9,6 +9,9 @@
 // formed in turns in fp64 -- pos * freq reaches 1e5 radians, where fp32 holds a few thousandths -- and reduced there, so
 // sine and cosine are fp32 functions of a number in -1/2..1/2.  A wave does all its heads of one row with one set of
 // sines; rows and heads are divided until about 8192 waves run, then a wave takes more heads of its row.
+//
+// Measured: 8192 rows of 32 + 8 heads of 128, f32, 336 MB read and written in 68-70 us = 4.8-4.9 TB/s (a copy of 256 MiB
+// runs at 5.4); one row 4.25 us, of which an empty launch is about 3.
 #include "internal.h"
 #include "kv_dev.h"
 

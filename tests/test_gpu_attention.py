@@ -396,6 +396,23 @@ def test_attention(ctx, lens, news, heads, kv_heads, dim, block, kind, options):
     _attend(ctx, np.random.default_rng(sum(lens) + dim), lens, news, heads, kv_heads, dim, block, kind, **options)
 
 
+SPLIT = [  # caches cut over many workgroups: lens, new rows, heads, kv_heads, dim, block, kind, options
+    ([33000], [1], 16, 1, 128, 64, "f32", {}),                                       # more splits than a round of the join takes
+    ([8100, 5000], [100, 62], 16, 4, 128, 64, "f32", {"sinks": True}),              # ten splits of 128 rows, many values to join
+    ([3000] * 3 + [0] * 20, [9, 1, 1] + [0] * 20, 8, 1, 64, 32, "f32", {}),          # one sequence of many more rows than most
+    ([3000] * 3 + [0] * 20, [9, 1, 1] + [0] * 20, 8, 1, 256, 16, "bf16", {"cap": 30.0, "sinks": True}),
+    ([2100], [17], 8, 2, 80, 64, "f16", {}),                                         # 68 rows: the least that goes by 128
+    ([2100], [16], 8, 2, 80, 64, "f16", {"sinks": True}),                            # 64 rows: the most that goes by 16
+    ([2100, 70], [17, 16], 8, 2, 80, 32, "f32", {}),                                 # both at once
+    ([5000] * 5, [1] * 5, 12, 3, 192, 64, "f32", {"window": 4000}),
+]
+
+
+@pytest.mark.parametrize("lens,news,heads,kv_heads,dim,block,kind,options", SPLIT)
+def test_attention_split_over_workgroups(ctx, lens, news, heads, kv_heads, dim, block, kind, options):
+    _attend(ctx, np.random.default_rng(sum(lens) * 3 + heads), lens, news, heads, kv_heads, dim, block, kind, **options)
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("new", [1, 100])
 @pytest.mark.parametrize("block", [16, 64])
