@@ -232,7 +232,7 @@ __device__ __forceinline__ float first_sum(const AttnLaunch &a, int lo, int hi) 
 // cache is split over workgroups a second kernel joins those.
 //
 // Measured, f32, 32 query and 8 key/value heads of 128: 64 sequences of up to 8192 tokens 154 us (754 MB, 4.9 TB/s; a copy
-// runs at 5.4); one sequence of 4096 tokens 7.2 us and 3.5 us for the second kernel.
+// runs at 5.4); one sequence of 4096 tokens 10.5 us (7.2 and the second kernel), of 32768 21.2 (3.2 TB/s), of 131072 50.3 (5.3).
 constexpr int ROWS = 16;
 
 struct RowsLds {
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
 // of one behind the other: the 1024 scores of 32 rows against 32 tokens alone are 16 matrix instructions (538 ns) and 128
 // vector instructions (289 ns), and both together measured 720 ns.
 //
-// Measured: 2 prompts of 4096 and 2506 tokens, bf16, 32 and 8 heads of 128: 245-253 us = 760-780 TFLOP/s (569 us the 16-row
+// Measured: 2 prompts of 4096 and 2577 tokens, bf16, 32 and 8 heads of 128: 245-253 us = 760-780 TFLOP/s (569 us the 16-row
 // way, which widens every code for 16 rows at a time); 2048 rows over 32768 tokens 860 TFLOP/s; a large library product
 // runs at 1200.  f32, whose products are taken twice: 509 rows over 16001 tokens, 16 and 8 heads of 256, capped, 367 us =
 // 358 TFLOP/s (715 executed; 333 us without the cap).
@@ -944,7 +944,7 @@ hipError_t launch_join(const AttnLaunch &a, const Share &share, hipStream_t s) {
     const int64_t rows = ((int64_t)a.b.n_rows * a.group + a.b.n_seqs - 1) / a.b.n_seqs, values = (rows < R ? rows : R) * (a.c.head_dim / 4);
     const auto grid = [&](int width) { return dim3((unsigned)share.items, (unsigned)a.c.kv_heads, (unsigned)((values + width - 1) / width)); };
     // eight threads for each value where one would not fill the device (two tiles of 8 heads in ten splits: 62.9 us the whole
-    // call with eight threads, 55.7 with one; 16 single tokens in five splits 27.0 and 28.6)
+    // call with eight threads, 55.7 with one)
     if (values * share.items * a.c.kv_heads > 65536) attn_join_kernel<T, R, 1><<<grid(256), 256, 0, s>>>(a);
     else attn_join_kernel<T, R, 8><<<grid(32), 256, 0, s>>>(a);
     return hipGetLastError();
