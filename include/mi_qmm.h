@@ -374,7 +374,8 @@ void mi_qmm_kv_free(mi_qmm_kv *kv);
  * With host arrays a page that is needed and outside 0..n_pages - 1, a length beyond the table, rows beyond the length or
  * row_start that falls or leaves 0..n is MI_QMM_ERR_INVALID.  With device arrays the call cannot see them: tokens of such
  * a page (or beyond the table) are not written, read back as NaN, and make every row that sees them NaN; rows whose
- * row_start is wrong, or whose position is negative, are left alone by write and read. */
+ * row_start is wrong, or whose position is negative, are left alone by write and read.
+ * At most 65536 sequences, and 2^24 pages in a table. */
 typedef struct mi_qmm_batch {
     int n_seqs, max_pages;
     const int32_t *row_start; /* [n_seqs + 1] */

@@ -2038,8 +2038,10 @@ hipError_t rows_to_host(void *host, const void *dev, int64_t n, int64_t stride, 
 
 int check_kv(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *b) {
     if (!kv || !b) return fail(MI_QMM_ERR_INVALID, "kv or batch is NULL");
-    if (b->n_seqs < 0 || b->max_pages < 1 || b->max_pages > (1 << 24) || b->n_seqs > (1 << 24))
-        return fail(MI_QMM_ERR_INVALID, "n_seqs=%d max_pages=%d", b->n_seqs, b->max_pages);
+    if (b->n_seqs < 0 || b->max_pages < 1) return fail(MI_QMM_ERR_INVALID, "n_seqs=%d max_pages=%d", b->n_seqs, b->max_pages);
+    // every workgroup looks for its sequence, 64 of them at a time
+    if (b->n_seqs > 65536 || b->max_pages > (1 << 24))
+        return fail(MI_QMM_ERR_UNSUPPORTED, "n_seqs=%d max_pages=%d: at most 65536 sequences and 2^24 pages each", b->n_seqs, b->max_pages);
     if (b->n_seqs && (!b->row_start || !b->kv_len || !b->pages)) return fail(MI_QMM_ERR_INVALID, "row_start, kv_len or pages is NULL");
     if (kv->device != ctx->device) return fail(MI_QMM_ERR_INVALID, "kv and ctx are on different devices");
     return MI_QMM_OK;

@@ -81,19 +81,35 @@ struct Found {
 
 // Work items numbered through the sequences, count(n, len) of them in a sequence of n rows and len tokens: where item
 // `item` falls.  A row range that is no part of 0..n_rows counts as none.  All lanes of a wave call it together; one round
-// of loads per 64 sequences.
+// of loads per 64 sequences, and while there are more than 256 ahead, one per 256 to pass over them (attention of 2048 single
+// tokens over up to 512: 530 -> 441 us).
 template <class F>
 __device__ __forceinline__ bool find_item(const DevBatch &b, int item, F count, Found &f) {
     const int lane = threadIdx.x & 63;
-    int base = 0;
-    for (int s0 = 0; s0 < b.n_seqs; s0 += 64) {
+    int base = 0, s0 = 0;
+    auto rows = [&](int begin, int end) { return begin >= 0 && end <= b.n_rows && end > begin ? end - begin : 0; };
+    for (; b.n_seqs - s0 > 256; s0 += 256) {
+        int begin[4], end[4], len[4], c = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int s = s0 + 64 * i + lane;
+            begin[i] = b.row_start[s];
+            end[i] = b.row_start[s + 1];
+            len[i] = b.kv_len[s];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) c += count(rows(begin[i], end[i]), max(len[i], 0));
+        const int total = __builtin_amdgcn_readlane(scan_add(c), 63);
+        if (item < base + total) break;
+        base += total;
+    }
+    for (; s0 < b.n_seqs; s0 += 64) {
         const int s = s0 + lane;
         int begin = 0, n = 0, len = 0, c = 0;
         if (s < b.n_seqs) {
             begin = b.row_start[s];
-            const int end = b.row_start[s + 1];
+            n = rows(begin, b.row_start[s + 1]);
             len = max(b.kv_len[s], 0);
-            n = begin >= 0 && end <= b.n_rows && end > begin ? end - begin : 0;
             c = count(n, len);
         }
         const int incl = scan_add(c);

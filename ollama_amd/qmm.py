@@ -490,8 +490,10 @@ class Context:
                             k_stride=None, q_out_stride=None, k_out_stride=None):
         """device pointers; strides in values from row to row (None: rows without gaps)"""
         q, k = heads.q_row, heads.k_row
-        rc = lib().mi_qmm_qk_norm_rope(self._h, heads._p, q_ptr, q_stride or q, k_ptr, k_stride or k, pos_ptr, n, q_out_ptr,
-                                       q_out_stride or q, k_out_ptr, k_out_stride or k, DEVICE)
+        rc = lib().mi_qmm_qk_norm_rope(self._h, heads._p, q_ptr, q if q_stride is None else q_stride, k_ptr,
+                                       k if k_stride is None else k_stride, pos_ptr, n, q_out_ptr,
+                                       q if q_out_stride is None else q_out_stride, k_out_ptr,
+                                       k if k_out_stride is None else k_out_stride, DEVICE)
         if rc:
             _check(rc)
 
@@ -537,18 +539,21 @@ class Context:
         return out
 
     def kv_write_device(self, kv: KVCache, batch: Batch, ggml_type: int, k_ptr, v_ptr, n: int, k_stride=None, v_stride=None):
-        rc = lib().mi_qmm_kv_write(self._h, kv._h, batch._p, ggml_type, k_ptr, k_stride or kv.row, v_ptr, v_stride or kv.row, n, DEVICE)
+        rc = lib().mi_qmm_kv_write(self._h, kv._h, batch._p, ggml_type, k_ptr, kv.row if k_stride is None else k_stride, v_ptr,
+                                   kv.row if v_stride is None else v_stride, n, DEVICE)
         if rc:
             _check(rc)
 
     def kv_read_device(self, kv: KVCache, batch: Batch, ggml_type: int, k_ptr, v_ptr, n: int, k_stride=None, v_stride=None):
-        rc = lib().mi_qmm_kv_read(self._h, kv._h, batch._p, ggml_type, k_ptr, k_stride or kv.row, v_ptr, v_stride or kv.row, n, DEVICE)
+        rc = lib().mi_qmm_kv_read(self._h, kv._h, batch._p, ggml_type, k_ptr, kv.row if k_stride is None else k_stride, v_ptr,
+                                   kv.row if v_stride is None else v_stride, n, DEVICE)
         if rc:
             _check(rc)
 
     def attention_device(self, kv: KVCache, batch: Batch, how: Attention, q_ptr, n: int, out_ptr, q_stride=None, out_stride=None):
         row = how.n_heads * kv.head_dim
-        rc = lib().mi_qmm_attention(self._h, kv._h, batch._p, how._p, q_ptr, q_stride or row, out_ptr, out_stride or row, n, DEVICE)
+        rc = lib().mi_qmm_attention(self._h, kv._h, batch._p, how._p, q_ptr, row if q_stride is None else q_stride, out_ptr,
+                                    row if out_stride is None else out_stride, n, DEVICE)
         if rc:
             _check(rc)
 

@@ -405,6 +405,8 @@ SPLIT = [  # caches cut over many workgroups: lens, new rows, heads, kv_heads, d
     ([2100], [16], 8, 2, 80, 64, "f16", {"sinks": True}),                            # 64 rows: the most that goes by 16
     ([2100, 70], [17, 16], 8, 2, 80, 32, "f32", {}),                                 # both at once
     ([5000] * 5, [1] * 5, 12, 3, 192, 64, "f32", {"window": 4000}),
+    ([i % 90 for i in range(1000)], [min(i % 90, i % 3) for i in range(1000)], 2, 1, 64, 32, "f32", {}),   # many sequences
+    ([40] * 257, [i % 2 for i in range(257)], 4, 2, 128, 64, "bf16", {}),
 ]
 
 
@@ -620,6 +622,10 @@ def test_refusals(ctx):
         nobody = qmm.Batch(1, 0, a.ptr, a.ptr, a.ptr)
         assert L.mi_qmm_attention(ctx._h, kv._h, nobody._p, how._p, a.ptr, 256, o.ptr, 256, 2, qmm.DEVICE) == qmm.ERR_INVALID
         assert L.mi_qmm_kv_read(ctx._h, kv._h, b._p, qmm.F32, a.ptr, 128, a.ptr + 256, 128, 2, qmm.DEVICE) == qmm.ERR_INVALID
+        for many in (qmm.Batch(65537, 2, a.ptr, a.ptr, a.ptr), qmm.Batch(1, (1 << 24) + 1, a.ptr, a.ptr, a.ptr)):
+            assert L.mi_qmm_attention(ctx._h, kv._h, many._p, how._p, a.ptr, 256, o.ptr, 256, 2, qmm.DEVICE) == qmm.ERR_UNSUPPORTED
+        with pytest.raises(qmm.QmmError):
+            ctx.attention_device(kv, b, how, a.ptr, 2, o.ptr, q_stride=0)
         none = qmm.Batch(0, 1, None, None, None)
         assert L.mi_qmm_attention(ctx._h, kv._h, none._p, how._p, a.ptr, 256, o.ptr, 256, 2, qmm.DEVICE) == 0
     # pages that a window leaves behind may be gone
