@@ -181,11 +181,22 @@ __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// x in a register of its own, copied here.  A register that a load of the loop's next round writes must not be handed on or
-// changed in place: the compiler then copies it at the end of the round, where that waits for the load just issued.
-__device__ __forceinline__ uint32_t copied(uint32_t x) {
-    uint32_t y;
-    asm("v_mov_b32 %0, %1" : "=v"(y) : "v"(x));
+// x and y in registers of their own, copied here.  A register that a load of the loop's next round writes must not be handed on
+// or changed in place: the compiler then copies it at the end of the round, where that waits for the load just issued.  The
+// two idle states belong to it: a lane swap must not follow within two instructions of the vector instruction that wrote its
+// register (a lane read not within one), and the compiler, which otherwise sees to that, does not look into the block.
+// Without them a swap now and then took what the register had held before: a wrong value code, and other bits on each call.
+__device__ __forceinline__ void copy_pair(uint32_t &x, uint32_t &y) {
+    uint32_t a, b;
+    asm("v_mov_b32 %0, %2\n\tv_mov_b32 %1, %3\n\ts_nop 1" : "=&v"(a), "=v"(b) : "v"(x), "v"(y));
+    x = a;
+    y = b;
+}
+
+// the same for one
+__device__ __forceinline__ float copied(float x) {
+    float y;
+    asm("v_mov_b32 %0, %1\n\ts_nop 1" : "=v"(y) : "v"(x));
     return y;
 }
 
@@ -585,8 +596,11 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
         for (int i = 0; i < NC; i++) {
             const int dt = wave * NC + i;
             // lanes 32 apart hold tokens 4 g .. and 4 (g + 2) .. of each 16: exchanged, each has both of two sixteens
-            const auto s0 = __builtin_amdgcn_permlane32_swap(copied(vc[i].x), copied(vc[i].z), false, false);
-            const auto s1 = __builtin_amdgcn_permlane32_swap(copied(vc[i].y), copied(vc[i].w), false, false);
+            uint32_t x0 = vc[i].x, z0 = vc[i].z, y0 = vc[i].y, w0 = vc[i].w;
+            copy_pair(x0, z0);
+            copy_pair(y0, w0);
+            const auto s0 = __builtin_amdgcn_permlane32_swap(x0, z0, false, false);
+            const auto s1 = __builtin_amdgcn_permlane32_swap(y0, w0, false, false);
             uint8_t *p = vb + (dt / 2 * 4 + lane / 32 * 2) * 1024 + ((g & 1) * 32 + (dt & 1) * 16 + x) * 16;
             *(half8 *)p = widen_centred(s0[0], s0[1]);
             *(half8 *)(p + 1024) = widen_centred(s1[0], s1[1]);
@@ -793,7 +807,7 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
         // goes on with pages that nobody works on (their number is the table's, or none: then page 0): without a condition
         // the loads go straight into the registers that the next round reads, with one they are waited for here.
         place(b ^ 1);
-        sc = __uint_as_float(copied(__float_as_uint(next_sc)));
+        sc = copied(next_sc);
         phys = next;
         const int k = page + 2 - t0;
         if (k % 64 == 0) ids = pages_from(a, seq, page + 2, 1);
