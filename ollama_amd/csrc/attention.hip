@@ -185,7 +185,7 @@ __device__ __forceinline__ void lds_barrier() {
 // or changed in place: the compiler then copies it at the end of the round, where that waits for the load just issued.  The
 // two idle states belong to it: a lane swap must not follow within two instructions of the vector instruction that wrote its
 // register (a lane read not within one), and the compiler, which otherwise sees to that, does not look into the block.
-// Without them a swap now and then took what the register had held before: a wrong value code, and other bits on each call.
+// Without them a swap may take what the register held before, which is another value's code.
 __device__ __forceinline__ void copy_pair(uint32_t &x, uint32_t &y) {
     uint32_t a, b;
     asm("v_mov_b32 %0, %2\n\tv_mov_b32 %1, %3\n\ts_nop 1" : "=&v"(a), "=v"(b) : "v"(x), "v"(y));
