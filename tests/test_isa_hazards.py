@@ -135,3 +135,10 @@ def test_registers_of_lane_swaps(built):
     assert any(SWAP.search(x) for x in lines) and any(DPP.search(x) for x in lines)  # the instructions in question are there
     found = [f for f in found if "its register" in f[1]]
     assert not found, f"{len(found)}, the first: {found[:5]}"
+
+
+def test_m0_of_loads_to_lds(built):
+    lines, found = built
+    assert any("_load_lds_" in x for x in lines)
+    found = [f for f in found if "m0" in f[1]]
+    assert not found, f"{len(found)}, the first: {found[:5]}"
