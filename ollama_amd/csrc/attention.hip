@@ -163,15 +163,18 @@ __device__ __forceinline__ float lane_float(float x, int lane) {
 }
 
 // as scalars; NaN where there is no such page: whoever sees it gets NaN.  Scales of 16 tokens that none of the rows worked on
-// together (lo .. hi - 1 for all of them) sees are 0: what stands there is a page's earlier content, and of any size.
-__device__ __forceinline__ void spread_scales(float &x, int phys, int j0, int lo, int hi, float (&ks)[4], float (&vs)[4]) {
+// together (lo .. hi - 1 for all of them) sees are 0: what stands there is a page's earlier content, and of any size.  Returns
+// whether one of the rows sees the lane's 16 tokens.
+__device__ __forceinline__ bool spread_scales(float &x, int phys, int j0, int lo, int hi, float (&ks)[4], float (&vs)[4]) {
     const int j = j0 + 16 * (threadIdx.x & 3);
-    x = j < hi && j + 16 > lo ? (phys < 0 ? __builtin_nanf("") : x) : 0.f;
+    const bool seen = j < hi && j + 16 > lo;
+    x = seen ? (phys < 0 ? __builtin_nanf("") : x) : 0.f;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
         ks[t] = lane_float(x, t);
         vs[t] = lane_float(x, 4 + t);
     }
+    return seen;
 }
 
 // A barrier for what the waves put into LDS alone: __syncthreads() would also wait for the loads of the page after next.
@@ -670,7 +673,7 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
         const int b = (page - t0) & 1;
         lds_barrier();
         const int j0 = page * KV_PAGE;
-        spread_scales(sc, phys, j0, w_lo_min, w_hi_max, ks, vs);
+        const bool seen = spread_scales(sc, phys, j0, w_lo_min, w_hi_max, ks, vs);
         const bool works = wrow0 < rows && j0 < w_hi_max && j0 + KV_PAGE > w_lo_min;  // else nothing that this wave's rows see
         if (works) {
         take_out_nan(ks, vs, j0, lo, hi, l);
@@ -750,9 +753,11 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
         const float base = m == MINUS_INF ? 0.f : m;
         Halves ph[4], pl[PHILO ? 4 : 1];
         // 16-bit calls: the value scale goes into the exponent and the sum of the probabilities comes back from the weighted
-        // ones -- while no scale is so far below the largest that halves would lose the sum.  A block of zeros may have any
-        // scale.  Logarithm and reciprocal of the page's scales are taken once, in the lanes that hold them.
-        const float wl = sc == 0.f ? ref * unit : sc * unit;
+        // ones -- while no scale is so far below the largest that halves would lose the sum.  Tokens that no row sees have
+        // probabilities of 0, whatever their weight; tokens that are seen under a scale of 0 count in the sum with a weight of
+        // 0, and a page with such takes the other way: their codes may be anything.  Logarithm and reciprocal of the page's
+        // scales are taken once, in the lanes that hold them.
+        const float wl = (seen ? sc : ref) * unit;
         if (!HILO && __ballot((lane & 4) && !(wl >= 0x1p-3f)) == 0) {
             const float log_w = __builtin_amdgcn_logf(wl), inv_w = __builtin_amdgcn_rcpf(wl);
             const half2v ones = {(_Float16)1.f, (_Float16)1.f};

@@ -4,7 +4,6 @@ import numpy as np
 import pytest
 
 import attnref
-from hipmem import DeviceArray
 from ollama_amd import qmm
 from test_gpu_attention import TYPES, Device, ctx, host  # noqa: F401
 
@@ -48,3 +47,51 @@ def test_the_same_bits_on_every_call(ctx, kind, dim, cap):  # noqa: F811
             kv.free()
     finally:
         other.close()
+
+def _defined(kind, want, bound, half):
+    """the bar of attnref's bound with the half steps of the output's type and of fp32"""
+    return bound + (half + 2.0 ** -24) * np.abs(want) + 2.0 ** -25 * (kind == "f16")
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new", [1, 3, 100, 180])
+@pytest.mark.parametrize("block", [16, 64])
+def test_blocks_of_scale_zero_hold_zeros(ctx, kind, new, block):  # noqa: F811
+    """tokens that were never written stand in cleared memory as code -128 under scale 0, or in a caller's as any code: their
+    values are 0 and their scores 0, and they take part in the sum"""
+    t, half = TYPES[kind]
+    rng = np.random.default_rng(new + block)
+    dim, heads, kv_heads, n = 64, 4, 2, 300
+    pages = rng.permutation(6)[:5].reshape(1, 5)
+    size, codes = qmm.kv_bytes(6, kv_heads, dim, block), 2 * 6 * kv_heads * 64 * dim
+    ref = attnref.Cache(6, kv_heads, dim, block)
+    k, v = rng.standard_normal((2, n, kv_heads, dim)).astype(np.float32)
+    with Device(ctx) as dev:
+        for cleared in (True, False):
+            used = np.zeros(size, np.uint8)
+            if not cleared:
+                used[:codes] = rng.integers(0, 256, codes)
+                for plane, place in zip(range(2), attnref.places(dim)):
+                    flat = used[plane * codes // 2:(plane + 1) * codes // 2].reshape(6, kv_heads, 64 * dim)
+                    ref.codes[plane][:] = flat[..., place.reshape(-1)].reshape(6, kv_heads, 64, dim).astype(np.int32) - 128
+            for s in ref.scales:
+                s[:] = 0
+            kv = ctx.kv_create(6, kv_heads, dim, block, memory=None if cleared else dev(used).ptr)
+            # the second page's, a part of the third's and the last tokens' blocks are written; the rest is not
+            for first, last in ((64, 128), (128, 160), (256, 300)):
+                b = qmm.Batch.of([0, last - first], [last], pages)
+                ctx.kv_write(kv, b, k[first:last], v[first:last])
+                ref.write([0, last - first], [last], pages, k[first:last], v[first:last])
+            gk, gv = ctx.kv_read(kv, qmm.Batch.of([0, n], [n], pages), n)
+            assert np.all(gv[:64] == 0) and np.all(gv[192:256] == 0) and np.all(np.abs(gv[256:300]).max(-1) > 0)
+            q, qv = dev.values(rng.standard_normal((new, heads, dim)), kind)
+            out = dev.values(np.zeros((new, heads, dim)), kind)[0]
+            b = qmm.Batch(1, 5, dev(np.array([0, new], np.int32)).ptr, dev(np.array([n], np.int32)).ptr, dev(pages, np.int32).ptr)
+            for window in (0, 90):
+                ctx.attention_device(kv, b, qmm.Attention(t, heads, 0.125, window), q.ptr, new, out.ptr)
+                ctx.sync()
+                want, bound = attnref.attention(ref, [0, new], [n], pages, qv, 0.125, window)
+                bar = _defined(kind, want, bound, half) + (np.abs(v).max() * 2.0 ** -11 if kind == "bf16" else 0)
+                err = np.abs(host(out, kind) - want)
+                assert np.all(err <= bar), (cleared, window, float(np.max(err / bar)))
+            kv.free()
