@@ -360,7 +360,8 @@ int mi_qmm_rope_freqs(int n_rot, double base, double freq_scale, double ext_fact
  * [n_pages][n_kv_heads][64 * dp], and lie inside a page and head at
  *     key   (token t, dimension d):  (((t / 16 * (dp / 64) + d / 64) * 4 + d % 64 / 16) * 16 + t % 16) * 16 + d % 16
  *     value (token t, dimension d):  ((d / 16 * 4 + t % 16 / 4) * 16 + d % 16) * 16 + t / 16 * 4 + t % 4
- * and scales are f32 [n_pages][n_kv_heads][64 / block]. */
+ * and scales are f32 [n_pages][n_kv_heads][64 / block], 0 or positive: attention takes a negative one like NaN (every row
+ * that sees one of the block's tokens is NaN).  Under a scale of 0 the codes may be anything. */
 #define MI_QMM_KV_PAGE 64
 typedef struct mi_qmm_kv mi_qmm_kv;
 int64_t mi_qmm_kv_bytes(int64_t n_pages, int n_kv_heads, int head_dim, int block); /* -1: no such cache */

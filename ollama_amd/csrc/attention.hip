@@ -162,13 +162,14 @@ __device__ __forceinline__ float lane_float(float x, int lane) {
     return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), lane));
 }
 
-// as scalars; NaN where there is no such page: whoever sees it gets NaN.  Scales of 16 tokens that none of the rows worked on
+// as scalars; NaN where there is no such page, and for a negative scale (the maxima below are taken before the key scales, and
+// the values' reference by the largest scale): whoever sees it gets NaN.  Scales of 16 tokens that none of the rows worked on
 // together (lo .. hi - 1 for all of them) sees are 0: what stands there is a page's earlier content, and of any size.  Returns
 // whether one of the rows sees the lane's 16 tokens.
 __device__ __forceinline__ bool spread_scales(float &x, int phys, int j0, int lo, int hi, float (&ks)[4], float (&vs)[4]) {
     const int j = j0 + 16 * (threadIdx.x & 3);
     const bool seen = j < hi && j + 16 > lo;
-    x = seen ? (phys < 0 ? __builtin_nanf("") : x) : 0.f;
+    x = seen ? (phys >= 0 && x >= 0.f ? x : __builtin_nanf("")) : 0.f;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
         ks[t] = lane_float(x, t);

@@ -95,3 +95,32 @@ def test_blocks_of_scale_zero_hold_zeros(ctx, kind, new, block):  # noqa: F811
                 err = np.abs(host(out, kind) - want)
                 assert np.all(err <= bar), (cleared, window, float(np.max(err / bar)))
             kv.free()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new", [1, 150])
+@pytest.mark.parametrize("plane", [0, 1])
+def test_negative_scales_count_as_no_number(ctx, kind, new, plane):  # noqa: F811
+    t, _ = TYPES[kind]
+    rng = np.random.default_rng(new)
+    with Device(ctx) as dev:
+        size, codes = qmm.kv_bytes(4, 1, 64, 64), 2 * 4 * 64 * 64
+        mem = dev(np.zeros(size, np.uint8))
+        kv = ctx.kv_create(4, 1, 64, 64, memory=mem.ptr)
+        k = rng.standard_normal((200, 1, 64)).astype(np.float32)
+        ctx.kv_write(kv, qmm.Batch.of([0, 200], [200], [[0, 1, 2, 3]]), k, k)
+        b = qmm.Batch(1, 4, dev(np.array([0, new], np.int32)).ptr, dev(np.array([200], np.int32)).ptr, dev(np.arange(4), np.int32).ptr)
+        q = dev.values(rng.standard_normal((new, 2, 64)), kind)[0]
+        raw = mem.numpy()
+        scales = raw[codes:].view(np.float32)
+        scales[4 * plane + 1] *= -1  # tokens 64 .. 127
+        mem.set(raw)
+        for window in (0, 73, 40):
+            out = dev.values(np.zeros((new, 2, 64)), kind)[0]
+            ctx.attention_device(kv, b, qmm.Attention(t, 2, 0.125, window), q.ptr, new, out.ptr)
+            ctx.sync()
+            at = np.arange(200 - new, 200)
+            sees = (at >= 64) & (at - (window or 1000) + 1 < 128)
+            got = host(out, kind)
+            assert np.isnan(got[sees]).all() and np.isfinite(got[~sees]).all()
+        kv.free()
