@@ -823,6 +823,7 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
     }
 
     l += other_half(l);
+    if (hi <= lo) l = 0.f;  // sees no token: zeros, also where its own infinities or NaN made the masked scores NaN
     if (!valid) return;
     const int o_h = head * a.group + my_h;
     const float base = m == MINUS_INF ? 0.f : m;

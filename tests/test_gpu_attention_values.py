@@ -124,3 +124,27 @@ def test_negative_scales_count_as_no_number(ctx, kind, new, plane):  # noqa: F81
             got = host(out, kind)
             assert np.isnan(got[sees]).all() and np.isfinite(got[~sees]).all()
         kv.free()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new", [40, 150])
+def test_rows_that_see_nothing_give_zeros_whatever_they_hold(ctx, kind, new):  # noqa: F811
+    """rows of negative positions (device arrays), their queries infinities and NaN"""
+    t, _ = TYPES[kind]
+    rng = np.random.default_rng(new)
+    for sinks in (False, True):
+        with Device(ctx) as dev:
+            kv = ctx.kv_create(2, 2, 64, 64)
+            k = rng.standard_normal((3, 2, 64)).astype(np.float32)
+            ctx.kv_write(kv, qmm.Batch.of([0, 3], [3], [[1]]), k, k)
+            x = rng.standard_normal((new, 4, 64)).astype(np.float32)
+            x[0::3, :, 5], x[1::3, :, 9], x[2:new - 3:3, :, 0] = np.nan, np.inf, -np.inf
+            x[new - 3:] = 1
+            q, out = dev.values(x, kind)[0], dev.values(np.full((new, 4, 64), 7.0), kind)[0]
+            how = qmm.Attention(t, 4, 0.125, sinks=dev(np.zeros(4, np.float32)).ptr if sinks else None)
+            b = qmm.Batch(1, 1, dev(np.array([0, new], np.int32)).ptr, dev(np.array([3], np.int32)).ptr, dev(np.array([[1]], np.int32)).ptr)
+            ctx.attention_device(kv, b, how, q.ptr, new, out.ptr)
+            ctx.sync()
+            got = host(out, kind)
+            assert np.all(got[:new - 3] == 0) and np.all(np.abs(got[new - 3:]).max(-1) > 0) and np.isfinite(got).all()
+            kv.free()
