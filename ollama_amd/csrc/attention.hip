@@ -165,11 +165,11 @@ __device__ __forceinline__ float lane_float(float x, int lane) {
 // as scalars; NaN where there is no such page, and for a negative scale (the maxima below are taken before the key scales, and
 // the values' reference by the largest scale): whoever sees it gets NaN.  Scales of 16 tokens that none of the rows worked on
 // together (lo .. hi - 1 for all of them) sees are 0: what stands there is a page's earlier content, and of any size.  Returns
-// whether one of the rows sees the lane's 16 tokens.
-__device__ __forceinline__ bool spread_scales(float &x, int phys, int j0, int lo, int hi, float (&ks)[4], float (&vs)[4]) {
+// whether one of the rows sees the lane's 16 tokens.  up: a factor of the lane's scale.
+__device__ __forceinline__ bool spread_scales(float &x, float up, int phys, int j0, int lo, int hi, float (&ks)[4], float (&vs)[4]) {
     const int j = j0 + 16 * (threadIdx.x & 3);
     const bool seen = j < hi && j + 16 > lo;
-    x = seen ? (phys >= 0 && x >= 0.f ? x : __builtin_nanf("")) : 0.f;
+    x = seen ? (phys >= 0 && x >= 0.f ? x * up : __builtin_nanf("")) : 0.f;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
         ks[t] = lane_float(x, t);
@@ -319,6 +319,7 @@ __device__ __forceinline__ void attn_rows(const AttnLaunch &a, RowsLds &lds, int
     // queries: dimensions 64 c + 16 g + 8 i .. + 7 of row r, as the second operand of step (c, i)
     Halves qh[2 * NC], ql[2 * NC];
     float score_scale, minus_bias;
+    float key_up = 1.f;  // lanes of key scales: the 2^24 of subnormal codes, where queries are so large that it has no room beside theirs
     {
         float x[NC][16];
         float big = 0.f;
@@ -331,8 +332,8 @@ __device__ __forceinline__ void attn_rows(const AttnLaunch &a, RowsLds &lds, int
             }
         big = fmaxf(big, __shfl_xor(big, 16));
         big = fmaxf(big, __shfl_xor(big, 32));
-        // the largest magnitude of a row to 2^13 .. 2^14: the halves keep 2^-38 of it
-        const int e = min(max(13 - exponent(big), -100), 100);
+        // the largest magnitude of a row to 2^13 .. 2^14 (for every finite one from 2^-87 on): the halves keep 2^-38 of it
+        const int e = min(max(13 - exponent(big), -115), 100);
         const float up = pow2(e);
         float sum = 0.f;
 #pragma unroll
@@ -352,7 +353,9 @@ __device__ __forceinline__ void attn_rows(const AttnLaunch &a, RowsLds &lds, int
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
         minus_bias = HILO ? 0.f : sum * (-128.f * 0x1p-24f);
-        score_scale = a.scale * (HILO ? 1.f : 0x1p24f) * pow2(-e) * (CAP ? 1.f / a.softcap : LOG2E);
+        const bool large = !HILO && __ballot(e < -64);
+        if (large && !(lane & 4)) key_up = 0x1p24f;
+        score_scale = a.scale * (HILO || large ? 1.f : 0x1p24f) * pow2(-e) * (CAP ? 1.f / a.softcap : LOG2E);
     }
 
     float4v acc[4 * NC];
@@ -369,7 +372,7 @@ __device__ __forceinline__ void attn_rows(const AttnLaunch &a, RowsLds &lds, int
         }
         float ks[4], vs[4];
         const int j0 = page * KV_PAGE;
-        spread_scales(sc, phys, j0, lo_min, hi_max, ks, vs);
+        spread_scales(sc, key_up, phys, j0, lo_min, hi_max, ks, vs);
         take_out_nan(ks, vs, j0, lo, hi, l);
         float z[16];
 #pragma unroll
@@ -616,7 +619,7 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
 
     // queries: dimensions 64 c + 16 (2 e + h) + 8 i .. + 7 of row r, as the second operand of step (c, e, i)
     Halves qh[NC][2][2], ql[HILO ? NC : 1][2][2];
-    float score_scale, minus_bias;
+    float score_scale, minus_bias, key_up = 1.f;  // (see the 16-row kernel)
     {
         float x[NC][2][16];
         float big = 0.f;
@@ -630,7 +633,7 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
                     big = fmaxf(big, fabsf(to_f32(raw[c][i][e])));
                 }
         big = fmaxf(big, other_half(big));
-        const int e = min(max(13 - exponent(big), -100), 100);
+        const int e = min(max(13 - exponent(big), -115), 100);
         const float up = a.scale < 0.f ? -pow2(e) : pow2(e);  // the scale's sign goes into the queries
         float sum = 0.f;
 #pragma unroll
@@ -645,7 +648,9 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
             }
         sum += other_half(sum);
         minus_bias = HILO ? 0.f : sum * (-128.f * 0x1p-24f);
-        score_scale = fabsf(a.scale) * (HILO ? 1.f : 0x1p24f) * pow2(-e) * (CAP ? 1.f / a.softcap : LOG2E);
+        const bool large = !HILO && __ballot(e < -64);
+        if (large && !(lane & 4)) key_up = 0x1p24f;
+        score_scale = fabsf(a.scale) * (HILO || large ? 1.f : 0x1p24f) * pow2(-e) * (CAP ? 1.f / a.softcap : LOG2E);
     }
 
     if constexpr (NC == 4) {
@@ -674,7 +679,7 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
         const int b = (page - t0) & 1;
         lds_barrier();
         const int j0 = page * KV_PAGE;
-        const bool seen = spread_scales(sc, phys, j0, w_lo_min, w_hi_max, ks, vs);
+        const bool seen = spread_scales(sc, key_up, phys, j0, w_lo_min, w_hi_max, ks, vs);
         const bool works = wrow0 < rows && j0 < w_hi_max && j0 + KV_PAGE > w_lo_min;  // else nothing that this wave's rows see
         if (works) {
         take_out_nan(ks, vs, j0, lo, hi, l);

@@ -148,3 +148,34 @@ def test_rows_that_see_nothing_give_zeros_whatever_they_hold(ctx, kind, new):  #
             got = host(out, kind)
             assert np.all(got[:new - 3] == 0) and np.all(np.abs(got[new - 3:]).max(-1) > 0) and np.isfinite(got).all()
             kv.free()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("size", [120, 126, -90, -110])
+def test_queries_at_the_ends_of_the_exponents(ctx, kind, new, size):  # noqa: F811
+    """queries around 2^size over keys around 2^-size: ordinary scores"""
+    t, half = TYPES[kind]
+    rng = np.random.default_rng(new)
+    n, dim = 200, 64
+    k = (rng.uniform(0.5, 1.9, (n, 1, dim)) * rng.choice([-1, 1], (n, 1, dim)) * 2.0 ** -size).astype(np.float32)
+    v = rng.standard_normal((n, 1, dim)).astype(np.float32)
+    ref = attnref.Cache(4, 1, dim, 64)
+    kv = ctx.kv_create(4, 1, dim, 64)
+    pages = [[2, 0, 1, 3]]
+    ctx.kv_write(kv, qmm.Batch.of([0, n], [n], pages), k, v)
+    ref.write([0, n], [n], pages, k, v)
+    with Device(ctx) as dev:
+        q, qv = dev.values((rng.uniform(0.5, 1.9, (new, 2, dim)) * rng.choice([-1, 1], (new, 2, dim)) * 2.0 ** size).astype(np.float32), kind)
+        out = dev.values(np.zeros((new, 2, dim)), kind)[0]
+        b = qmm.Batch(1, 4, dev(np.array([0, new], np.int32)).ptr, dev(np.array([n], np.int32)).ptr, dev(pages, np.int32).ptr)
+        ctx.attention_device(kv, b, qmm.Attention(t, 2, 0.125), q.ptr, new, out.ptr)
+        ctx.sync()
+        with np.errstate(over="ignore"):  # its bound adds a least scale of 1e-30, far above these: formed here as there, from the scales
+            want, _ = attnref.attention(ref, [0, new], [n], pages, qv, 0.125)
+        magnitudes = float(np.abs(qv.astype(np.float64)).sum(-1).max()) * 0.125 * 1.4427 * 256 * float(ref.scales[0].max())
+        assert 20 < magnitudes < 120
+        d = 2.0 ** -24 * (4 + 32) * magnitudes
+        own = np.abs(v).max() * (2 * (2.0 ** d - 1 + 2.0 ** -20) + (2.0 ** -11 if kind == "bf16" else 0))
+        assert np.all(np.abs(host(out, kind) - want) <= own + (half + 2.0 ** -24) * np.abs(want))
+    kv.free()
