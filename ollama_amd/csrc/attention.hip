@@ -18,6 +18,8 @@
 //   per pair (left in, 128 would make sum p (code + 128) hundreds of times the result)
 //   scales of keys multiply the scores; scales of values the probabilities, against a running power of two so that the
 //   product is at most 1
+#include <atomic>
+
 #include "internal.h"
 #include "kv_dev.h"
 
@@ -990,12 +992,17 @@ hipError_t launch_one(const AttnLaunch &a, hipStream_t s) {
         constexpr int lds = 2 * 4 * KV_PAGE * 64 * NC;
         static_assert(lds >= (int)sizeof(RowsLds), "the 16-row way shares the buffers");
         if constexpr (lds > 65536) {
-            static bool allowed[2][64] = {};  // more than 64 KiB of dynamic LDS has to be allowed once per device
+            // More than 64 KiB of dynamic LDS has to be allowed once per device: a bit for each, set by whichever thread comes
+            // first (two at once both ask for it, which does no harm); devices without a bit are asked for on every call.
+            static std::atomic<uint64_t> allowed[2];
             int dev = 0;
-            if (hipGetDevice(&dev) == hipSuccess && dev >= 0 && dev < 64 && !allowed[a.softcap > 0.f][dev]) {
-                const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+            hipError_t e = hipGetDevice(&dev);
+            if (e != hipSuccess) return e;
+            const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+            if (!(allowed[a.softcap > 0.f].load(std::memory_order_relaxed) & bit)) {
+                e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
                 if (e != hipSuccess) return e;
-                allowed[a.softcap > 0.f][dev] = true;
+                allowed[a.softcap > 0.f].fetch_or(bit, std::memory_order_relaxed);
             }
         }
         kernel<<<few + many, 256, lds, s>>>(a);

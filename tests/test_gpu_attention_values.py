@@ -1,5 +1,7 @@
 """Attention over the 8-bit cache: the same bits on every call, and the results that the definition gives where cache contents
 or arguments are out of the ordinary.  Restatement and bars as in test_gpu_attention.py."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -179,3 +181,35 @@ def test_queries_at_the_ends_of_the_exponents(ctx, kind, new, size):  # noqa: F8
         own = np.abs(v).max() * (2 * (2.0 ** d - 1 + 2.0 ** -20) + (2.0 ** -11 if kind == "bf16" else 0))
         assert np.all(np.abs(host(out, kind) - want) <= own + (half + 2.0 ** -24) * np.abs(want))
     kv.free()
+
+
+@pytest.mark.parametrize("dim", [192, 256])
+def test_first_calls_of_several_threads(dim):
+    """a context per thread, all at their first prompt of a head size whose kernel asks for its LDS once per device"""
+    rng = np.random.default_rng(dim)
+    n, kinds = 150, ["f32", "f16"]
+    k, v = rng.standard_normal((2, n, 1, dim)).astype(np.float32)
+    ref = attnref.Cache(3, 1, dim, 64)
+    ref.write([0, n], [n], [[2, 0, 1]], k, v)
+    start, got = threading.Barrier(4), {}
+
+    def work(i):
+        with qmm.Context(0) as c:
+            kv = c.kv_create(3, 1, dim, 64)
+            b = qmm.Batch.of([0, n], [n], [[2, 0, 1]])
+            c.kv_write(kv, b, k, v)
+            q = np.random.default_rng(i).standard_normal((n, 2, dim)).astype(np.float32 if kinds[i % 2] == "f32" else np.float16)
+            start.wait(60)
+            got[i] = q, c.attention(kv, b, q, 0.0625, softcap=30.0 * (i // 2))
+            kv.free()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert sorted(got) == [0, 1, 2, 3]
+    for i, (q, out) in got.items():
+        want, bound = attnref.attention(ref, [0, n], [n], [[2, 0, 1]], q, 0.0625, cap=30.0 * (i // 2))
+        kind = kinds[i % 2]
+        assert np.all(np.abs(out.astype(np.float64) - want) <= _defined(kind, want, bound, TYPES[kind][1]))
