@@ -399,7 +399,7 @@ int mi_qmm_kv_read(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *bat
  *     out = sum_j w_j v_j / (sum_j w_j + exp(sink)),  w_j = exp(z_j),  z_j = cap(scale * q . k_j),  cap(z) = c tanh(z / c)
  * over the tokens j of the row's sequence with j <= its position (causal) and j > its position - window (window > 0).
  * Query head h reads key/value head h / (n_heads / n_kv_heads).  sinks: one logit per query head that takes part in the
- * sum only; softcap 0: no cap; scale and softcap are finite.  A row that sees no token gives zeros.  f32 calls carry f32
+ * sum only; softcap 0: no cap, otherwise 2^-64 .. 2^64; scale is finite.  A row that sees no token gives zeros.  f32 calls carry f32
  * accuracy (queries and probabilities are split into two halves each); the 16-bit types take probabilities of 11 bits
  * (f16 of 22).  A value's share (its weight times its scale) is rounded at 2^-34 of the largest value scale among the
  * tokens that the 128 (token, head) rows worked on together see, so scales that far apart do not add up to f32 accuracy.

@@ -2295,6 +2295,9 @@ int mi_qmm_attention(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *b
     if (!(p->softcap >= 0.f) || p->window < 0) return fail(MI_QMM_ERR_INVALID, "softcap=%g window=%d must be non-negative", (double)p->softcap, p->window);
     if (!std::isfinite(p->scale) || !std::isfinite(p->softcap))
         return fail(MI_QMM_ERR_INVALID, "scale=%g softcap=%g must be finite", (double)p->scale, (double)p->softcap);
+    // scores are formed in units of the cap, times its reciprocal
+    if (p->softcap != 0.f && (p->softcap < 0x1p-64f || p->softcap > 0x1p64f))
+        return fail(MI_QMM_ERR_UNSUPPORTED, "softcap=%g: 0 or from 2^-64 to 2^64", (double)p->softcap);
     // a launch has at most 2^24 workgroups of 256: 16 rows each, one more per sequence and head
     if (n * p->n_heads + 15 * std::min<int64_t>(n, b->n_seqs) * c.kv_heads > (1 << 27))
         return fail(MI_QMM_ERR_UNSUPPORTED, "n=%lld rows of %d heads in %d sequences", (long long)n, p->n_heads, b->n_seqs);

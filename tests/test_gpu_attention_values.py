@@ -213,3 +213,30 @@ def test_first_calls_of_several_threads(dim):
         want, bound = attnref.attention(ref, [0, n], [n], [[2, 0, 1]], q, 0.0625, cap=30.0 * (i // 2))
         kind = kinds[i % 2]
         assert np.all(np.abs(out.astype(np.float64) - want) <= _defined(kind, want, bound, TYPES[kind][1]))
+
+
+def test_caps_from_the_smallest_to_the_largest(ctx):  # noqa: F811
+    """2^-64 and 2^64 hold; beyond them a score in units of the cap, or the cap itself in units of log2, leaves fp32: refused"""
+    rng = np.random.default_rng(1)
+    n, dim = 130, 64
+    k, v = rng.standard_normal((2, n, 1, dim)).astype(np.float32)
+    ref = attnref.Cache(3, 1, dim, 64)
+    kv = ctx.kv_create(3, 1, dim, 64)
+    b = qmm.Batch.of([0, n], [n], [[2, 0, 1]])
+    ctx.kv_write(kv, b, k, v)
+    ref.write([0, n], [n], [[2, 0, 1]], k, v)
+    for new in (1, n):
+        rows = qmm.Batch.of([0, new], [n], [[2, 0, 1]])
+        for kind in (np.float32, np.float16):
+            q = rng.standard_normal((new, 2, dim)).astype(kind)
+            q[0, 0] = 0  # scores of 0 stay 0 under every cap
+            for cap in (2.0 ** -64, 1e-6, 1e6, 2.0 ** 64):
+                got = ctx.attention(kv, rows, q, 0.125, softcap=cap).astype(np.float64)
+                want, bound = attnref.attention(ref, [0, new], [n], [[2, 0, 1]], q, 0.125, cap=cap)
+                name = "f32" if kind is np.float32 else "f16"
+                assert np.all(np.abs(got - want) <= _defined(name, want, bound, TYPES[name][1])), (new, kind, cap)
+            for cap in (3e38, 1e38, 2.0 ** 65, 2.0 ** -65, 1e-39, 1e-45):
+                with pytest.raises(qmm.QmmError) as e:
+                    ctx.attention(kv, rows, q, 0.125, softcap=cap)
+                assert e.value.code == qmm.ERR_UNSUPPORTED
+    kv.free()
