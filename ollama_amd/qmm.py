@@ -265,7 +265,8 @@ class QKHeads:
 
 class Batch:
     """The sequences of a step (mi_qmm_batch): device addresses of row_start int32 [n_seqs + 1], kv_len int32 [n_seqs]
-    and pages int32 [n_seqs][max_pages]; or, from numpy arrays, host ones (Batch.of)."""
+    and pages int32 [n_seqs][max_pages], for the _device calls; or, from numpy arrays, host ones (Batch.of), for the calls
+    with host arrays."""
 
     def __init__(self, n_seqs: int, max_pages: int, row_start_ptr, kv_len_ptr, pages_ptr):
         self._s = _Batch(n_seqs, max_pages, row_start_ptr, kv_len_ptr, pages_ptr)
@@ -281,6 +282,12 @@ class Batch:
         b = cls(pages.shape[0], pages.shape[1], row_start.ctypes.data, kv_len.ctypes.data, pages.ctypes.data)
         b._keep = (row_start, kv_len, pages)
         return b
+
+    def _at(self, host: bool):
+        """the struct's address for a call with host (or device) arrays: the other kind's addresses would be read by the wrong side"""
+        if (self._keep is not None) != host:
+            raise ValueError("this call wants a batch of host arrays (Batch.of)" if host else "this call wants a batch of device addresses, not Batch.of")
+        return self._p
 
 
 class Attention:
@@ -514,13 +521,13 @@ class Context:
         self._kv_shape(kv, k, "k")
         if v.shape != k.shape or v.dtype != k.dtype:
             raise ValueError(f"k {k.shape} {k.dtype} and v {v.shape} {v.dtype} differ")
-        _check(lib().mi_qmm_kv_write(self._h, kv._h, batch._p, _value_type(k), _ptr(k), kv.row, _ptr(v), kv.row, k.shape[0], HOST))
+        _check(lib().mi_qmm_kv_write(self._h, kv._h, batch._at(True), _value_type(k), _ptr(k), kv.row, _ptr(v), kv.row, k.shape[0], HOST))
 
     def kv_read(self, kv: KVCache, batch: Batch, n: int, dtype=np.float32):
         """(k, v) [n, kv_heads, dim] of the batch's rows (host); rows of no sequence are zeros"""
         k = np.zeros((n, kv.n_kv_heads, kv.head_dim), dtype)
         v = np.zeros_like(k)
-        _check(lib().mi_qmm_kv_read(self._h, kv._h, batch._p, _value_type(k), _ptr(k), kv.row, _ptr(v), kv.row, n, HOST))
+        _check(lib().mi_qmm_kv_read(self._h, kv._h, batch._at(True), _value_type(k), _ptr(k), kv.row, _ptr(v), kv.row, n, HOST))
         return k, v
 
     def attention(self, kv: KVCache, batch: Batch, q: np.ndarray, scale: float, window: int = 0, softcap: float = 0.0,
@@ -535,24 +542,24 @@ class Context:
                 raise ValueError(f"sinks {sinks.shape}, q has {q.shape[1]} heads")
         how = Attention(_value_type(q), q.shape[1], scale, window, softcap, None if sinks is None else sinks.ctypes.data, causal)
         out, row = np.zeros_like(q), q.shape[1] * q.shape[2]
-        _check(lib().mi_qmm_attention(self._h, kv._h, batch._p, how._p, _ptr(q), row, _ptr(out), row, q.shape[0], HOST))
+        _check(lib().mi_qmm_attention(self._h, kv._h, batch._at(True), how._p, _ptr(q), row, _ptr(out), row, q.shape[0], HOST))
         return out
 
     def kv_write_device(self, kv: KVCache, batch: Batch, ggml_type: int, k_ptr, v_ptr, n: int, k_stride=None, v_stride=None):
-        rc = lib().mi_qmm_kv_write(self._h, kv._h, batch._p, ggml_type, k_ptr, kv.row if k_stride is None else k_stride, v_ptr,
+        rc = lib().mi_qmm_kv_write(self._h, kv._h, batch._at(False), ggml_type, k_ptr, kv.row if k_stride is None else k_stride, v_ptr,
                                    kv.row if v_stride is None else v_stride, n, DEVICE)
         if rc:
             _check(rc)
 
     def kv_read_device(self, kv: KVCache, batch: Batch, ggml_type: int, k_ptr, v_ptr, n: int, k_stride=None, v_stride=None):
-        rc = lib().mi_qmm_kv_read(self._h, kv._h, batch._p, ggml_type, k_ptr, kv.row if k_stride is None else k_stride, v_ptr,
+        rc = lib().mi_qmm_kv_read(self._h, kv._h, batch._at(False), ggml_type, k_ptr, kv.row if k_stride is None else k_stride, v_ptr,
                                    kv.row if v_stride is None else v_stride, n, DEVICE)
         if rc:
             _check(rc)
 
     def attention_device(self, kv: KVCache, batch: Batch, how: Attention, q_ptr, n: int, out_ptr, q_stride=None, out_stride=None):
         row = how.n_heads * kv.head_dim
-        rc = lib().mi_qmm_attention(self._h, kv._h, batch._p, how._p, q_ptr, row if q_stride is None else q_stride, out_ptr,
+        rc = lib().mi_qmm_attention(self._h, kv._h, batch._at(False), how._p, q_ptr, row if q_stride is None else q_stride, out_ptr,
                                     row if out_stride is None else out_stride, n, DEVICE)
         if rc:
             _check(rc)

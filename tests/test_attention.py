@@ -144,3 +144,20 @@ def test_python_side_shape_checks():
     assert b._s.n_seqs == 1 and b._s.max_pages == 2
     with pytest.raises(TypeError):
         qmm._value_type(np.zeros(1))
+
+
+def test_batches_of_the_wrong_side_are_refused():
+    """host addresses never reach a kernel, device addresses never the host's checks"""
+    kv = qmm.KVCache(None, 1, 1, 8, 64)
+    ctx = qmm.Context.__new__(qmm.Context)
+    ctx._h = None
+    host, device = qmm.Batch.of([0, 1], [1], [[0]]), qmm.Batch(1, 1, 4096, 4096, 4096)
+    x, how = np.zeros((1, 1, 8), np.float32), qmm.Attention(qmm.F32, 1, 1.0)
+    for call in (lambda: ctx.kv_write(kv, device, x, x), lambda: ctx.kv_read(kv, device, 1), lambda: ctx.attention(kv, device, x, 1.0),
+                 lambda: ctx.kv_write_device(kv, host, qmm.F32, 4096, 4096, 1), lambda: ctx.kv_read_device(kv, host, qmm.F32, 4096, 4096, 1),
+                 lambda: ctx.attention_device(kv, host, how, 4096, 1, 4096)):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: ctx.kv_write(kv, host, x, x), lambda: ctx.attention_device(kv, device, how, 4096, 1, 4096)):
+        with pytest.raises(qmm.QmmError):  # these come as far as the missing context
+            call()
