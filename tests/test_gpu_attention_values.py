@@ -240,3 +240,117 @@ def test_caps_from_the_smallest_to_the_largest(ctx):  # noqa: F811
                     ctx.attention(kv, rows, q, 0.125, softcap=cap)
                 assert e.value.code == qmm.ERR_UNSUPPORTED
     kv.free()
+
+
+
+@pytest.mark.parametrize("new", [1, 4, 70])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scores_that_are_small_differences_f16(ctx, new, dim):  # noqa: F811
+    """whole-number queries and keys, so that every product and partial sum of a score is a whole number below 2^24 and fp32
+    holds it: what a score may lose is its own rounding, not one of the magnitudes that it is the difference of.  The tokens
+    are picked so that their scores lie within a few units of each other, far below those magnitudes (300 in log2)."""
+    rng = np.random.default_rng(new + dim)
+    n, heads, block = 192, 4, 64
+    pages = rng.permutation(4)[:3].reshape(1, 3)
+    q = np.zeros((new, heads, dim), np.float16)
+    k = np.zeros((n, heads, dim), np.float32)
+    for h in range(heads):
+        q[:, h] = rng.integers(-255, 256, dim)
+        codes = rng.integers(-127, 128, (400000, dim))
+        codes[:, 7] = 127  # every block's scale is 1 to a rounding
+        score = codes @ q[0, h].astype(np.int64)
+        k[:, h] = codes[rng.permutation(np.argsort(np.abs(score - 2 * score.std()))[:n])]
+    v = rng.standard_normal((n, heads, dim)).astype(np.float32)
+    ref = attnref.Cache(4, heads, dim, block)
+    kv = ctx.kv_create(4, heads, dim, block)
+    b = qmm.Batch.of([0, n], [n], pages)
+    ctx.kv_write(kv, b, k, v)
+    ref.write([0, n], [n], pages, k, v)
+    assert np.array_equal(ref.codes[0][pages[0]].transpose(0, 2, 1, 3).reshape(n, heads, dim), k)
+    magnitudes = np.abs(q[0].astype(np.float64)).sum(-1).max() * 64 * 1.4427
+    scale = np.float32(300 / magnitudes)
+    got = ctx.attention(kv, qmm.Batch.of([0, new], [n], pages), q, float(scale)).astype(np.float64)
+    want, _ = attnref.attention(ref, [0, new], [n], pages, q, np.float64(scale))
+    # scores in units of log2 up to |z|: the product with its factor, the factor's own three roundings, the difference to the
+    # maximum: 5 half steps of |z|; the weights' and sums' own 2^-20 on top, half a step of f16 and one of its subnormals
+    z = max(np.abs(k[:, h].astype(np.float64) @ q[0, h].astype(np.float64)).max() for h in range(heads)) * float(scale) * 1.4427
+    bar = np.abs(v).max() * 2 * (2.0 ** (5 * 2.0 ** -24 * z) - 1 + 2.0 ** -20) + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
+    err = np.abs(got - want)
+    assert np.all(err <= bar), float(np.max(err / bar))
+    kv.free()
+
+
+@pytest.mark.parametrize("new", [1, 4, 100])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_f16_takes_probabilities_of_22_bits(ctx, new, dim):  # noqa: F811
+    """no term for a rounding of the probabilities to 11 bits: attnref's bound and the output's half step, where scores are of
+    one dimension (a bound of 1e-5) and six values of either sign cancel (the half step is small too).  Probabilities of 11
+    bits are off by 7 to 21 of these bars."""
+    rng = np.random.default_rng(new + dim)
+    half = TYPES["f16"][1]
+    n, heads, kv_heads, window = 200, 8, 2, 6
+    k, v = np.zeros((n, kv_heads, dim), np.float32), rng.choice([-1, 1], (n, kv_heads, dim)) * rng.uniform(0.7, 1, (n, 1, 1))
+    k[..., 0] = rng.uniform(-1, 1, (n, kv_heads))
+    q = np.zeros((new, heads, dim), np.float16)
+    q[..., 0] = rng.uniform(0.5, 1.5, (new, heads))
+    ref = attnref.Cache(4, kv_heads, dim, 16)
+    kv = ctx.kv_create(4, kv_heads, dim, 16)
+    pages = [[2, 0, 1, 3]]
+    ctx.kv_write(kv, qmm.Batch.of([0, n], [n], pages), k, v.astype(np.float32))
+    ref.write([0, n], [n], pages, k, v.astype(np.float32))
+    got = ctx.attention(kv, qmm.Batch.of([0, new], [n], pages), q, 1.0, window).astype(np.float64)
+    want, bound = attnref.attention(ref, [0, new], [n], pages, q, 1.0, window)
+    assert bound.max() < 2e-5 and (np.abs(want) < 2.0 ** -5).any()
+    assert np.all(np.abs(got - want) <= _defined("f16", want, bound, half))
+    kv.free()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("gap", [6, 16, 20])
+def test_small_values_beside_large_ones_without_weight(ctx, kind, new, block, gap):  # noqa: F811
+    """one block in two holds values 2^gap larger under scores so low that it has no weight: the result has the small values'
+    size.  A share is rounded at 2^-34 of the largest value scale that a tile sees, or is less than that itself; what is lost
+    of a row is at most the sum over its tokens, times 127 codes."""
+    t, half = TYPES[kind]
+    rng = np.random.default_rng(new + block + gap)
+    n, dim, heads = 400, 64, 2
+    big = np.arange(n) // block % 2 == 1
+    k = rng.standard_normal((n, 1, dim)) * 0.05
+    k[:, 0, 0] = np.where(big, -8.0, 8.0)
+    k[:, 0, 1] = rng.standard_normal(n)
+    v = rng.standard_normal((n, 1, dim)) * np.where(big, 2.0 ** gap, 1.0)[:, None, None]
+    k, v = k.astype(np.float32), v.astype(np.float32)
+    pages = rng.permutation(8)[:7].reshape(1, 7)
+    ref = attnref.Cache(8, 1, dim, block)
+    kv = ctx.kv_create(8, 1, dim, block)
+    ctx.kv_write(kv, qmm.Batch.of([0, n], [n], pages), k, v)
+    ref.write([0, n], [n], pages, k, v)
+    with Device(ctx) as dev:
+        x = rng.standard_normal((new, heads, dim)) * 0.1
+        x[..., 0], x[..., 1] = 16, 6  # scores of -128 and of 128 +- 18: the large values' weights are below e^-200
+        q, qv = dev.values(x, kind)
+        out = dev.values(np.zeros((new, heads, dim)), kind)[0]
+        b = qmm.Batch(1, 7, dev(np.array([0, new], np.int32)).ptr, dev(np.array([n], np.int32)).ptr, dev(pages, np.int32).ptr)
+        ctx.attention_device(kv, b, qmm.Attention(t, heads, 1.0), q.ptr, new, out.ptr)
+        ctx.sync()
+        want, _ = attnref.attention(ref, [0, new], [n], pages, qv, 1.0)
+        step = 2.0 ** -33 * float(ref.scales[1].max())  # the kernel's reference is a power of two, up to twice the largest scale
+        kk = ref.values(pages[0], n)[0][:, 0]
+        z = np.einsum("nhd,md->nhm", qv.astype(np.float64), kk)
+        z[:, :, big] = -np.inf
+        z = np.where(np.arange(n)[None, None, :] <= np.arange(n - new, n)[:, None, None], z, -np.inf)
+        w = np.exp(z - z.max(-1, keepdims=True))
+        w /= w.sum(-1, keepdims=True)
+        scales = np.repeat(np.concatenate([ref.scales[1][p, 0] for p in pages[0]]), block)[:n].astype(np.float64)
+        lost = 127 * np.minimum(step, w * scales).sum(-1)[..., None]
+        # scores: 6e-6 of the magnitudes that make them (subnormal key codes; bf16), 64 half steps of them otherwise; a
+        # probability's own 2^-12 (bf16); the output's half step
+        small = float(np.abs(v[~big]).max())
+        d = (8e-6 if kind == "bf16" else 2.0 ** -18) * 1.4427 * (128 + 18 + 12)
+        own = small * (2 * (2.0 ** d - 1 + 2.0 ** -20) + (2.0 ** -11 if kind == "bf16" else 0))
+        err, bar = np.abs(host(out, kind) - want), lost + own + (half + 2.0 ** -24) * np.abs(want) + 2.0 ** -25 * (kind == "f16")
+        assert np.sqrt(np.mean(want ** 2)) > 5 * bar.max()  # the bar would see the small values lost
+        assert np.all(err <= bar), (float(np.max(err / bar)), float(lost.max()), own)
+    kv.free()
