@@ -111,6 +111,12 @@ __device__ __forceinline__ float other_half(float x) {
     return __uint_as_float(threadIdx.x & 32 ? r[0] : r[1]);
 }
 
+// a head's sink in units of log2; what overflows there, infinity too, counts as the largest number: all weight is the sink's
+__device__ __forceinline__ float sink_of(const AttnLaunch &a, int head) {
+    const float x = a.sinks[head] * LOG2E;
+    return x > 0x1.fffffep127f ? 0x1.fffffep127f : x;
+}
+
 __device__ __forceinline__ void visible(const AttnLaunch &a, int pos, int len, int &lo, int &hi) {
     lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
     hi = a.causal ? min(pos + 1, len) : len;
@@ -474,7 +480,7 @@ __device__ __forceinline__ void attn_rows(const AttnLaunch &a, RowsLds &lds, int
     if (a.few.splits == 1) {
         float total = sum;
         if (a.sinks) {
-            const float sink = a.sinks[o_h] * LOG2E, all = fmaxf(base, sink);
+            const float sink = sink_of(a, o_h), all = fmaxf(base, sink);
             // the sink joins the sum; where it is the largest, everything is measured against it
             divide = __builtin_amdgcn_exp2f(base - all);
             total = sum * divide + __builtin_amdgcn_exp2f(sink - all);
@@ -840,7 +846,7 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
     if (a.many.splits == 1) {
         float total = l, scale = 1.f;
         if (a.sinks) {
-            const float sink = a.sinks[o_h] * LOG2E, all = fmaxf(base, sink);
+            const float sink = sink_of(a, o_h), all = fmaxf(base, sink);
             scale = __builtin_amdgcn_exp2f(base - all);
             total = l * scale + __builtin_amdgcn_exp2f(sink - all);
         }
@@ -905,7 +911,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnLaunch a) {
         const bool live = i < rows * quads;
         const int row = live ? divided(i, a.by_quads) : 0, d = live ? (i - row * quads) * 4 : 0;
         const int t = divided(tile * R + row, a.by_group), h = head * a.group + tile * R + row - t * a.group;
-        const float sink = a.sinks ? a.sinks[h] * LOG2E : MINUS_INF;
+        const float sink = a.sinks ? sink_of(a, h) : MINUS_INF;
         float top = MINUS_INF, sum = 0.f;
         float4v y = {0.f, 0.f, 0.f, 0.f};
         // what a further part of the row adds: maximum m, sum l, numerators x; one that saw nothing has no numerators

@@ -354,3 +354,32 @@ def test_small_values_beside_large_ones_without_weight(ctx, kind, new, block, ga
         assert np.sqrt(np.mean(want ** 2)) > 5 * bar.max()  # the bar would see the small values lost
         assert np.all(err <= bar), (float(np.max(err / bar)), float(lost.max()), own)
     kv.free()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,new", [(200, 1), (200, 150), (9000, 1), (9000, 20)])
+def test_sinks_from_the_lowest_to_the_largest(ctx, kind, n, new):  # noqa: F811
+    """minus infinity and the lowest numbers: as without a sink; the largest and infinity take all the weight: zeros"""
+    t, half = TYPES[kind]
+    rng = np.random.default_rng(n + new)
+    table = -(-n // 64)
+    pages = rng.permutation(table).reshape(1, table)
+    k, v = rng.standard_normal((2, n, 1, 64)).astype(np.float32)
+    sinks = np.array([-np.inf, -3e38, -1e4, 0.5, 1e4, 3e38, np.inf, np.nan], np.float32)
+    kv = ctx.kv_create(table, 1, 64, 64)
+    ctx.kv_write(kv, qmm.Batch.of([0, n], [n], pages), k, v)
+    with Device(ctx) as dev:
+        q = dev.values(rng.standard_normal((new, 8, 64)), kind)[0]
+        b = qmm.Batch(1, table, dev(np.array([0, new], np.int32)).ptr, dev(np.array([n], np.int32)).ptr, dev(pages, np.int32).ptr)
+        got = []
+        for s in (None, dev(sinks).ptr):
+            out = dev.values(np.zeros((new, 8, 64)), kind)[0]
+            ctx.attention_device(kv, b, qmm.Attention(t, 8, 0.125, sinks=s), q.ptr, new, out.ptr)
+            ctx.sync()
+            got.append(host(out, kind))
+        assert np.array_equal(got[0][:, :3], got[1][:, :3]) and np.isfinite(got[1][:, :7]).all()
+        # the sink of 0.5 takes 1.6 / 9000 = 2^-12.4 of the weight there, less than half a step of the 16-bit types: the rounded
+        # result is smaller or the same, never larger
+        assert np.all(np.abs(got[1][:, 3]) <= np.abs(got[0][:, 3])) and np.all(got[1][:, 4:7] == 0)
+        assert np.isnan(got[1][:, 7]).all()
+    kv.free()
