@@ -118,7 +118,7 @@ __device__ __forceinline__ float sink_of(const AttnLaunch &a, int head) {
 }
 
 __device__ __forceinline__ void visible(const AttnLaunch &a, int pos, int len, int &lo, int &hi) {
-    lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    lo = a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0;  // (pos may be negative, and the window 2^31 - 1)
     hi = a.causal ? min(pos + 1, len) : len;
     hi = max(hi, 0);
 }

@@ -383,3 +383,28 @@ def test_sinks_from_the_lowest_to_the_largest(ctx, kind, n, new):  # noqa: F811
         assert np.all(np.abs(got[1][:, 3]) <= np.abs(got[0][:, 3])) and np.all(got[1][:, 4:7] == 0)
         assert np.isnan(got[1][:, 7]).all()
     kv.free()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("new", [3, 40, 150])
+def test_the_largest_window_is_none(ctx, causal, new):  # noqa: F811
+    """rows of negative positions among them: position less window stays in range, and the bits are those without a window"""
+    rng = np.random.default_rng(new)
+    kv = ctx.kv_create(3, 1, 64, 64)
+    n = 130
+    k, v = rng.standard_normal((2, n, 1, 64)).astype(np.float32)
+    ctx.kv_write(kv, qmm.Batch.of([0, n], [n], [[2, 0, 1]]), k, v)
+    with Device(ctx) as dev:
+        q = dev.values(rng.standard_normal((2 * new, 2, 64)), "f32")[0]
+        lens = dev(np.array([2, n], np.int32))
+        b = qmm.Batch(2, 3, dev(np.array([0, new, 2 * new], np.int32)).ptr, lens.ptr, dev(np.array([[2, 0, 1]] * 2, np.int32)).ptr)
+        got = []
+        for window in (0, 2 ** 31 - 1, 2 ** 31 - 200):
+            out = dev.values(np.full((2 * new, 2, 64), 7.0), "f32")[0]
+            ctx.attention_device(kv, b, qmm.Attention(qmm.F32, 2, 0.125, window, causal=causal), q.ptr, 2 * new, out.ptr)
+            ctx.sync()
+            got.append(out.numpy())
+        assert np.isfinite(got[0]).all() and np.abs(got[0][new:]).max() > 0.01
+        assert not causal or np.all(got[0][: new - 2] == 0)
+        assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+    kv.free()
