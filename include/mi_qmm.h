@@ -346,7 +346,7 @@ int mi_qmm_qk_norm_rope(mi_qmm_ctx *ctx, const mi_qmm_qk_heads *heads, const voi
                         int64_t k_stride, const int32_t *pos, int64_t n, void *q_out, int64_t q_out_stride, void *k_out,
                         int64_t k_out_stride, int location);
 /* Fills freqs (HOST memory, n_rot / 2 doubles) and mscale; needs no GPU.  freq_i = base^(-2 i / n_rot) / factors[i]
- * (factors may be NULL), times freq_scale (linear scaling); with ext_factor != 0 the published YaRN rule: dimensions that
+ * (factors may be NULL; positive and finite), times freq_scale (linear scaling); with ext_factor != 0 the published YaRN rule: dimensions that
  * turn more than beta_fast times within n_ctx_orig positions keep their frequency, those below beta_slow turns take the
  * scaled one, a ramp between; mscale = attn_factor * (1 + 0.1 ln(1 / freq_scale)).  Without it mscale = attn_factor. */
 int mi_qmm_rope_freqs(int n_rot, double base, double freq_scale, double ext_factor, double attn_factor, double beta_fast,

@@ -2096,6 +2096,11 @@ int mi_qmm_rope_freqs(int n_rot, double base, double freq_scale, double ext_fact
     if (n_rot < 2 || n_rot % 2) return fail(MI_QMM_ERR_INVALID, "n_rot=%d must be even and positive", n_rot);
     if (!(base > 1.0) || !(freq_scale > 0.0)) return fail(MI_QMM_ERR_INVALID, "base=%g must be above 1 and freq_scale=%g positive", base, freq_scale);
     if (!freqs || !mscale) return fail(MI_QMM_ERR_INVALID, "freqs or mscale is NULL");
+    if (!std::isfinite(base) || !std::isfinite(freq_scale) || !std::isfinite(ext_factor) || !std::isfinite(attn_factor))
+        return fail(MI_QMM_ERR_INVALID, "base=%g freq_scale=%g ext_factor=%g attn_factor=%g must be finite", base, freq_scale, ext_factor, attn_factor);
+    for (int i = 0; factors && i < n_rot / 2; i++)
+        if (!(factors[i] > 0.f) || !std::isfinite(factors[i]))
+            return fail(MI_QMM_ERR_INVALID, "factors[%d]=%g must be positive and finite", i, (double)factors[i]);
     const bool yarn = ext_factor != 0.0;
     if (yarn && (n_ctx_orig < 1 || !(beta_fast > 0.0) || !(beta_slow > 0.0)))
         return fail(MI_QMM_ERR_INVALID, "n_ctx_orig=%d beta_fast=%g beta_slow=%g must be positive", n_ctx_orig, beta_fast, beta_slow);

@@ -161,3 +161,15 @@ def test_batches_of_the_wrong_side_are_refused():
     for call in (lambda: ctx.kv_write(kv, host, x, x), lambda: ctx.attention_device(kv, device, how, 4096, 1, 4096)):
         with pytest.raises(qmm.QmmError):  # these come as far as the missing context
             call()
+
+
+def test_rope_freqs_of_no_numbers_are_refused():
+    """an infinite frequency would turn position 0 into NaN; nothing is written"""
+    for bad in (dict(base=np.inf), dict(base=np.nan), dict(freq_scale=np.inf), dict(freq_scale=np.nan), dict(attn_factor=np.nan),
+                dict(ext_factor=np.nan, n_ctx_orig=4096), dict(factors=[1, 0, 1, 1]), dict(factors=[1, 1, 1, -2]), dict(factors=[np.nan, 1, 1, 1]),
+                dict(factors=[1, np.inf, 1, 1])):
+        with pytest.raises(qmm.QmmError) as e:
+            qmm.rope_freqs(8, **{"base": 1e4, **bad})
+        assert e.value.code == qmm.ERR_INVALID, bad
+    f, m = qmm.rope_freqs(8, 1e4, factors=[1, 2, 4, 1e30])
+    assert np.isfinite(f).all() and (f > 0).all() and m == 1.0
