@@ -361,7 +361,7 @@ __device__ __forceinline__ void attn_rows(const AttnLaunch &a, RowsLds &lds, int
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
         minus_bias = HILO ? 0.f : sum * (-128.f * 0x1p-24f);
-        const bool large = !HILO && __ballot(e < -64);
+        const bool large = __is_same(T, __bf16) && __ballot(e < -64);  // (f16 ends at 2^16)
         if (large && !(lane & 4)) key_up = 0x1p24f;
         score_scale = a.scale * (HILO || large ? 1.f : 0x1p24f) * pow2(-e) * (CAP ? 1.f / a.softcap : LOG2E);
     }
@@ -656,7 +656,7 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
             }
         sum += other_half(sum);
         minus_bias = HILO ? 0.f : sum * (-128.f * 0x1p-24f);
-        const bool large = !HILO && __ballot(e < -64);
+        const bool large = __is_same(T, __bf16) && __ballot(e < -64);
         if (large && !(lane & 4)) key_up = 0x1p24f;
         score_scale = fabsf(a.scale) * (HILO || large ? 1.f : 0x1p24f) * pow2(-e) * (CAP ? 1.f / a.softcap : LOG2E);
     }
