@@ -399,10 +399,13 @@ int mi_qmm_kv_read(mi_qmm_ctx *ctx, const mi_qmm_kv *kv, const mi_qmm_batch *bat
  *     out = sum_j w_j v_j / (sum_j w_j + exp(sink)),  w_j = exp(z_j),  z_j = cap(scale * q . k_j),  cap(z) = c tanh(z / c)
  * over the tokens j of the row's sequence with j <= its position (causal) and j > its position - window (window > 0).
  * Query head h reads key/value head h / (n_heads / n_kv_heads).  sinks: one logit per query head that takes part in the
- * sum only; softcap 0: no cap, otherwise 2^-64 .. 2^64; scale is finite.  A row that sees no token gives zeros.  f32 calls carry f32
- * accuracy (queries and probabilities are split into two halves each); the 16-bit types take probabilities of 11 bits
- * (f16 of 22).  A value's share (its weight times its scale) is rounded at 2^-34 of the largest value scale among the
- * tokens that the 128 (token, head) rows worked on together see, so scales that far apart do not add up to f32 accuracy.
+ * sum only (minus infinity: no sink; what leaves fp32 in units of log2 takes all the weight); softcap 0: no cap, otherwise
+ * 2^-64 .. 2^64; scale is finite.  A row that sees no token gives zeros.
+ * f32 calls carry f32 accuracy (queries and probabilities are split into two halves each).  f16 takes probabilities of 22
+ * bits, bf16 of 11: an error of 1.7e-4 of an output's size before the output's own rounding of 1.7e-3; a bf16 caller who
+ * wants less makes an f32 call.  Both take a score to 6e-6 of its size.  A value's share (its weight times its scale) is
+ * rounded at 2^-34 of the largest value scale among the tokens that the 128 (token, head) rows worked on together see, so
+ * scales that far apart do not add up to f32 accuracy.
  * The rows' own tokens are to be written first (mi_qmm_kv_write on the same batch).  q, out [n][n_heads][head_dim], not
  * overlapping. */
 typedef struct mi_qmm_attn {

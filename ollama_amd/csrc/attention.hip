@@ -12,8 +12,9 @@
 // of the lane, and the probabilities are already the second product's operand.
 //   key codes of 16-bit calls as subnormal halves (code + 128) 2^-24, one byte permute per pair: the accumulators start at
 //   -128 2^-24 sum q, which takes the 128 out.  The matrix cores align a product by its operands' exponent fields, and a
-//   subnormal's is that of 2^-14: ten bits of the sum are lost, 6e-6 of a score (measured), nothing to 16-bit results but
-//   too much for f32
+//   subnormal's is that of 2^-14: ten bits of the sum are lost, 6e-6 of a score (measured on ordinary scores; where scores
+//   lie within a few units of each other and are differences of magnitudes of 300, in units of log2, f16 outputs are no
+//   more than 1.5e-6 beyond their half step, of values up to 4, against 1e-6 for f32 calls).  Too much for f32
 //   key codes of f32 calls, and value codes, as the whole numbers themselves: 1024 + byte less 1152, one more instruction
 //   per pair (left in, 128 would make sum p (code + 128) hundreds of times the result)
 //   scales of keys multiply the scores; scales of values the probabilities, against a running power of two so that the
@@ -254,8 +255,10 @@ __device__ __forceinline__ float first_sum(const AttnLaunch &a, int lo, int hi) 
 // waves of a workgroup every fourth one, each with its own running maximum; the workgroup joins them, and where the
 // cache is split over workgroups a second kernel joins those.
 //
-// Measured, f32, 32 query and 8 key/value heads of 128: 64 sequences of up to 8192 tokens 154 us (754 MB, 4.9 TB/s; a copy
-// runs at 5.4); one sequence of 4096 tokens 10.5 us (7.2 and the second kernel), of 32768 21.2 (3.2 TB/s), of 131072 50.3 (5.3).
+// Measured, f32, 32 query and 8 key/value heads of 128: 64 sequences of up to 8192 tokens 153 us (754 MB, 4.9 TB/s; a copy
+// runs at 5.4), bf16 150; one sequence of 4096 tokens 10.7 us (7.3 and the second kernel), of 32768 21.2 (3.2 TB/s), of 131072
+// 50.3 (5.3).  Heads of 192 and 256 fill the registers with a page, so that one wave runs per SIMD and nothing hides its page's
+// arithmetic: 16 sequences of up to 8192 tokens, 16 and 8 heads of 256, 89 us (393 MB, 4.4 TB/s), one of 32768 42 (3.2).
 constexpr int ROWS = 16;
 
 struct RowsLds {
@@ -532,14 +535,19 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
 // Bound: the vector ALU beside the matrix cores.  A wave holds 32 rows, the workgroup's four waves share each page of 64
 // tokens through LDS: each widens a quarter of the codes, once for all 128 rows, while the matrix instructions of the page
 // before run (two buffers; the codes are in registers one page ahead of that).  The exponentials of the softmax and the
-// widening take the vector ALU about as long as the products take the matrix cores, and two waves per SIMD hide only part
-// of one behind the other: the 1024 scores of 32 rows against 32 tokens alone are 16 matrix instructions (538 ns) and 128
-// vector instructions (289 ns), and both together measured 720 ns.
+// widening take the vector ALU about as long as the products take the matrix cores, and a wave does one after the other: scores,
+// softmax and the second product of a page in turn, held apart by a scheduling barrier, and two waves per SIMD (one at heads of
+// 192 and 256) hide only part of one behind the other.  The 1024 scores of 32 rows against 32 tokens alone are 16 matrix
+// instructions (538 ns) and 128 vector instructions (289 ns), and both together measured 720 ns.  This is how the kernel is
+// ordered, no limit of the machine: scores of the next page beside this page's softmax in one wave have not been tried.
 //
-// Measured: 2 prompts of 4096 and 2577 tokens, bf16, 32 and 8 heads of 128: 245-253 us = 760-780 TFLOP/s (569 us the 16-row
-// way, which widens every code for 16 rows at a time); 2048 rows over 32768 tokens 860 TFLOP/s; a large library product
-// runs at 1200.  f32, whose products are taken twice: 509 rows over 16001 tokens, 16 and 8 heads of 256, capped, 367 us =
-// 358 TFLOP/s (715 executed; 333 us without the cap).
+// Registers: no spills in bf16 at heads of 128; 10 at heads of 64 (see the launch bounds below); f16 at heads of 128 spills 17
+// (capped 11), f32 capped there 9; f32 at heads of 256 spills 24 (100 bytes per lane), capped 57 (228 bytes), inside the page loop.
+//
+// Measured: 2 prompts of 4096 and 2577 tokens, 32 and 8 heads of 128: bf16 244-255 us = 750-786 TFLOP/s (569 us the 16-row
+// way, which widens every code for 16 rows at a time), f16 330, f32 372; 2048 rows over 32768 tokens, bf16, 860 TFLOP/s; a large
+// library product runs at 1200.  509 rows over 16001 tokens, 16 and 8 heads of 256, capped: f32, whose products are taken
+// twice, 354 us = 371 TFLOP/s (742 executed), f16 268, bf16 226.
 constexpr int TILE = 128;
 constexpr float LAZY = 6.f;
 
@@ -878,8 +886,9 @@ __device__ __forceinline__ void attn_tile(const AttnLaunch &a, uint8_t *lds, int
 
 // Prompts, and in the same launch the sequences of few rows beside them: those first, so that single tokens are done while
 // the prompts are worked on.
-// Waves per SIMD: what the accumulators and queries leave; at heads of 64 three fit in bf16 (2048 rows over 2048 tokens of 64
-// heads 81.7 -> 76.5 us) but spill where probabilities are in two halves (f16 88.7 -> 94.6, capped 110 -> 4448).
+// Waves per SIMD: what the accumulators and queries leave; at heads of 64 three in bf16 pay, with ten spilled registers (2048
+// rows over 2048 tokens of 64 heads 81.7 -> 76.5 us), but not where probabilities are in two halves (f16 88.7 -> 94.6, capped
+// 110 -> 4448).
 template <class T, int NC, bool CAP>
 __global__ __launch_bounds__(256, NC == 1 && __is_same(T, __bf16) ? 3 : NC <= 2 ? 2 : 1) void attn_tile_kernel(AttnLaunch a) {
     extern __shared__ __align__(1024) uint8_t lds[];  // two buffers of a page's keys and values as halves
@@ -1049,7 +1058,9 @@ int splits_for(int64_t most, int64_t pages, double page_us, double bytes) {
     return best;
 }
 
-// Both shares with their splits; part is left to the caller.  floats: the partial results of each.
+// Both shares with their splits; part is left to the caller.  floats: the partial results of each.  The host knows the width
+// of the page table, not the lengths, and plans with it: 512 fresh rows of 32 / 8 heads of 128 are done in one piece under a table
+// of 8 pages (21.9 us) and in four under one of 2048 (32.4); a single token over 4096 takes 11.8 and 11.5.
 void shares_of(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus, Share &few, Share &many, size_t floats[2]) {
     const int64_t group = d.n_heads / c.kv_heads, all = b.n_rows * group;
     const int64_t active = b.n_seqs < b.n_rows ? b.n_seqs : b.n_rows;
@@ -1071,10 +1082,13 @@ void shares_of(const DevKv &c, const DevBatch &b, const AttnDesc &d, int num_cus
             const int64_t cap = active * ((FEW + ROWS - 1) / ROWS);
             if (items > cap) items = cap;
             // beside prompts: 64 pages per workgroup (16 rounds of its four waves, about 20 us) are done before a prompt is,
-            // and up to that length no second launch has to join anything
+            // and up to that length no second launch has to join anything.  The host does not see whether one of the sequences is
+            // a prompt, so steps of a few tokens each come here too once they are more than 64 rows: 10 sequences over up to
+            // 8192 tokens, 8 / 1 heads of 128, take 14.8 us with one token each, 37.5 with two
             want = (pages_seen(ROWS) + 63) / 64;
         } else {
-            // the workgroups that run at a time (three per CU at heads of 64, else two), down to a page per wave.  f32, 8
+            // the workgroups that run at a time (three per CU at heads of 64, two at 128; at 192 and 256 one runs, and the second
+            // half of the splits a second round), down to a page per wave.  f32, 8
             // heads of 128, two / eight per CU: one sequence of 32768 tokens 21.2 / 24.3 us, of 131072 49.8 / 55.5; 16 of up
             // to 4096 tokens in 3 / 4 / 5 splits 31.1 / 27.0 / 29.9, 32 of up to 8192 in 1 / 2 / 3 80.9 / 83.8 / 88.3
             want = (c.dp <= 64 ? 3ll : 2ll) * num_cus / (likely(ROWS, active) * c.kv_heads);

@@ -57,7 +57,7 @@ __device__ __forceinline__ int scan_add(int x) {
     return x;
 }
 
-// Division by a number that the host knows: 0 <= x < 2^31, 1 <= d < 2^31.  Three instructions, scalar ones where x is the
+// Division by a number that the host knows (Granlund and Montgomery 1994): 0 <= x < 2^31, 1 <= d < 2^31.  Three instructions, scalar ones where x is the
 // same for a wave; the general division is about forty vector instructions (and as much code to fetch).
 struct Divisor {
     uint32_t mul, shift;

@@ -11,8 +11,10 @@
 // through LDS, and a lane holds whole 16-byte value pieces; key codes are turned into their pieces through LDS.
 //
 // Measured, 8 heads of 128, f32: the write of 64 single tokens 4.6 us (7.9 before few tokens had a way of their own), the
-// write and read-back of 6091 tokens of four prompts 35 us (126 MB, 3.6 TB/s; the read alone runs at 4.9), the read of
-// 65536 tokens as bf16 82 us (403 MB, 4.9 TB/s; a copy 5.4).
+// write and read-back of 6091 tokens of four prompts 34-36 us (126 MB, 3.6 TB/s; the read alone runs at 4.9; a workgroup's load,
+// maximum and store of its page follow each other with nothing in flight behind them), as bf16 38 (75 MB, 2.0); the read of 65536
+// tokens as bf16 82 us (403 MB, 4.9 TB/s; a copy 5.4).  At heads of 256 66 us (251 MB), at heads of up to 64 52 us for half the
+// bytes of 128: that instance of the write takes 222 registers, two waves per SIMD, where the one for 128 takes 72.
 #include "internal.h"
 #include "kv_dev.h"
 
