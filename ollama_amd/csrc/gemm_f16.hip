@@ -69,17 +69,19 @@ __device__ __forceinline__ const uint8_t *uniform_ptr(const uint8_t *p) {
     const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
     return (const uint8_t *)(((unsigned long long)hi << 32) | lo);
 }
-// direct-to-LDS copy of 64 x 16 (64 x 4) bytes: lane l's piece of base + off lands at lds_addr + 16 l (4 l); m0 has to be
-// written one wait state before the load that takes its LDS address from it
+// direct-to-LDS copy of 64 x 16 (64 x 4) bytes: lane l's piece of base + off lands at lds_addr + 16 l (4 l)
+// Wait states: one between the write of m0 and the load to LDS, five between a scalar register's write by the vector ALU
+// (v_readfirstlane, right before as the compiler likes it) and a load that takes its base from it; the compiler keeps such
+// distances everywhere but around inline assembly
 __device__ __forceinline__ void dma16(const uint8_t *base, unsigned off, unsigned lds_addr) {
     base = uniform_ptr(base);
     lds_addr = __builtin_amdgcn_readfirstlane(lds_addr);
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_addr) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_addr) : "memory");
 }
 __device__ __forceinline__ void dma4(const uint8_t *base, unsigned off, unsigned lds_addr) {
     base = uniform_ptr(base);
     lds_addr = __builtin_amdgcn_readfirstlane(lds_addr);
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds_addr) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds_addr) : "memory");
 }
 // wait until at most N vector-memory operations of this wave are outstanding (they retire in order)
 template <int N>

@@ -129,14 +129,14 @@ __device__ __forceinline__ void dma_lds16(const uint8_t *base, unsigned off, uns
     const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
     const uint8_t *b = (const uint8_t *)(((unsigned long long)hi << 32) | lo);
     lds_addr = __builtin_amdgcn_readfirstlane(lds_addr);
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(b), "s"(lds_addr) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(b), "s"(lds_addr) : "memory");
 }
 __device__ __forceinline__ void dma_lds4(const uint8_t *base, unsigned off, unsigned lds_addr) {
     const unsigned long long v = (unsigned long long)base;
     const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
     const uint8_t *b = (const uint8_t *)(((unsigned long long)hi << 32) | lo);
     lds_addr = __builtin_amdgcn_readfirstlane(lds_addr);
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(b), "s"(lds_addr) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(b), "s"(lds_addr) : "memory");
 }
 
 struct CopyArgs {

@@ -60,6 +60,9 @@ __device__ __forceinline__ T lds_at(unsigned address, int imm) {
     return *(const __attribute__((address_space(3))) T *)(uintptr_t)(address + (unsigned)imm);
 }
 // direct-to-LDS copy issued from inline assembly: lane l's BYTES at base + off land at lds_address + BYTES * l
+// Wait states: one between the write of m0 and the load to LDS, five between a scalar register's write by the vector ALU
+// (v_readfirstlane, right before as the compiler likes it) and a load that takes its base from it; the compiler keeps such
+// distances everywhere but around inline assembly
 template <int BYTES>
 __device__ __forceinline__ void dma_lds(const uint8_t *base, unsigned off, unsigned lds_address) {
     const unsigned long long v = (unsigned long long)base;
@@ -67,9 +70,9 @@ __device__ __forceinline__ void dma_lds(const uint8_t *base, unsigned off, unsig
     base = (const uint8_t *)(((unsigned long long)hi << 32) | lo);
     lds_address = __builtin_amdgcn_readfirstlane(lds_address);
     if (BYTES == 16)
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_address) : "memory");
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_address) : "memory");
     else
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds_address) : "memory");
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds_address) : "memory");
 }
 __device__ __forceinline__ u4v bperm(int idx, u4v v) {
     u4v o;

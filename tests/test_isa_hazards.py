@@ -40,6 +40,14 @@ def registers(operand):
     return set(range(int(m.group(1)), int(m.group(2)) + 1)) if m else set()
 
 
+def scalars(text):
+    """the scalar registers that operands name"""
+    found = {int(x) for x in re.findall(r"\bs(\d+)\b", text)}
+    for a, b in re.findall(r"\bs\[(\d+):(\d+)\]", text):
+        found |= set(range(int(a), int(b) + 1))
+    return found
+
+
 SWAP = re.compile(r"v_permlane(16|32)_swap")
 DPP = re.compile(r"\b(quad_perm|row_shl|row_shr|row_ror|row_bcast|row_mirror|row_half_mirror|wave_\w+|row_newbcast)\b")
 
@@ -47,8 +55,10 @@ DPP = re.compile(r"\b(quad_perm|row_shl|row_shr|row_ror|row_bcast|row_mirror|row
 def hazards(lines):
     """(function, what is too close) for every violation; the distances of the published tables, in wait states:
     a vector register written by the vector ALU -> read by a lane swap or through a lane permutation (dpp): 2;
+    a scalar register written by the vector ALU -> read by a vector memory instruction: 5;
     m0 written -> a load that goes to LDS: 1"""
-    function, recent, found = None, [], []  # recent: (wait states it takes, registers written by the vector ALU, writes m0)
+    # recent: (wait states it takes, vector and scalar registers written by the vector ALU, writes m0)
+    function, recent, found = None, [], []
     for line in lines:
         if line.endswith(">:"):
             function, recent = line.split("<", 1)[-1][:-2], []
@@ -61,7 +71,7 @@ def hazards(lines):
             recent = []
             continue
         if op == "s_nop":
-            recent = (recent + [(int(rest, 0) + 1, set(), False)])[-4:]
+            recent = (recent + [(int(rest, 0) + 1, set(), set(), False)])[-6:]
             continue
         args = [a.strip() for a in rest.split(",")]
         if args:
@@ -72,17 +82,24 @@ def hazards(lines):
         elif op.startswith("v_") and DPP.search(rest):
             reads, need = registers(args[1].split(" ")[0]), 2
         to_lds = "_lds_" in op or (op.startswith("buffer_load") and rest.endswith(" lds"))
+        bases = scalars(rest) if op.startswith(("global_", "buffer_", "flat_", "scratch_")) else set()
         distance = 0
-        for states, written, m0 in reversed(recent):
+        for states, written, scalar, m0 in reversed(recent):
+            if distance < 5 and scalar & bases:
+                found.append((function, f"{text}: its base was written {distance} wait states before"))
             if distance < need and written & reads:
                 found.append((function, f"{text}: its register was written {distance} wait states before"))
             if distance < 1 and m0 and to_lds:
                 found.append((function, f"{text}: m0 was written right before"))
             distance += states
-        written = set()
+        written, scalar = set(), set()
+        if op.startswith(("v_readlane", "v_readfirstlane", "v_cmp")):
+            scalar = scalars(args[0])
+        elif op.startswith("v_") and len(args) > 1:  # a carry or a scale flag
+            scalar = scalars(args[1]) if re.match(r"v_(add|sub|subrev)_co|v_(addc|subb|subbrev)_co|v_div_scale|v_mad_[ui]64", op) else set()
         if op.startswith("v_") and not op.startswith(("v_cmp", "v_mfma", "v_smfma", "v_readlane", "v_readfirstlane")):
             written = registers(args[0]) | (registers(args[1]) if SWAP.match(op) else set())
-        recent = (recent + [(1, written, op.startswith("s_") and args[:1] == ["m0"])])[-4:]
+        recent = (recent + [(1, written, scalar, op.startswith("s_") and args[:1] == ["m0"])])[-6:]
     return found
 
 
@@ -109,10 +126,19 @@ def test_the_check_sees_what_it_looks_for():
 \ts_nop 1
 \tv_mov_b32_dpp v4, v1 row_shr:1 row_mask:0xf bank_mask:0xf
 \tv_mfma_f32_16x16x32_f16 v[0:3], v[4:7], v[8:11], v[0:3]
+0000000000003000 <h>:
+\tv_readfirstlane_b32 s7, v109
+\ts_mov_b32 m0, s4
+\ts_nop 2
+\tglobal_load_lds_dwordx4 v175, s[6:7]
+\tv_readfirstlane_b32 s6, v109
+\ts_mov_b32 m0, s4
+\ts_nop 3
+\tglobal_load_lds_dwordx4 v175, s[6:7]
 """
     found = hazards(code.splitlines())
-    assert [f for f, _ in found] == ["f"] * 3
-    assert "v66, v67" in found[0][1] and "m0" in found[1][1] and "row_shr" in found[2][1]
+    assert [f for f, _ in found] == ["f"] * 3 + ["h"]
+    assert "v66, v67" in found[0][1] and "m0" in found[1][1] and "row_shr" in found[2][1] and "base was written 4" in found[3][1]
 
 
 @pytest.fixture(scope="module")
@@ -141,4 +167,10 @@ def test_m0_of_loads_to_lds(built):
     lines, found = built
     assert any("_load_lds_" in x for x in lines)
     found = [f for f in found if "m0" in f[1]]
+    assert not found, f"{len(found)}, the first: {found[:5]}"
+
+
+def test_bases_of_vector_memory(built):
+    lines, found = built
+    found = [f for f in found if "its base" in f[1]]
     assert not found, f"{len(found)}, the first: {found[:5]}"
