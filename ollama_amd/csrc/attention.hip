@@ -544,7 +544,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(AttnLaunch a) {
 // Registers: no spills in bf16 at heads of 128; 10 at heads of 64 (see the launch bounds below); f16 at heads of 128 spills 17
 // (capped 11), f32 capped there 9; f32 at heads of 256 spills 24 (100 bytes per lane), capped 57 (228 bytes), inside the page loop.
 //
-// Measured: 2 prompts of 4096 and 2577 tokens, 32 and 8 heads of 128: bf16 244-255 us = 750-786 TFLOP/s (569 us the 16-row
+// Measured: 2 prompts of 4096 and 2577 tokens, 32 and 8 heads of 128: bf16 244-260 us = 740-786 TFLOP/s (569 us the 16-row
 // way, which widens every code for 16 rows at a time), f16 330, f32 372; 2048 rows over 32768 tokens, bf16, 860 TFLOP/s; a large
 // library product runs at 1200.  509 rows over 16001 tokens, 16 and 8 heads of 256, capped: f32, whose products are taken
 // twice, 354 us = 371 TFLOP/s (742 executed), f16 268, bf16 226.
